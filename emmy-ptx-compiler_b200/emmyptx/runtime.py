@@ -7,7 +7,9 @@ path: without the library, or without a CUDA device, every call raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libemmyb200.so"
@@ -64,6 +66,17 @@ class PwProgram(ctypes.Structure):
                 ("in_div", ctypes.c_int64 * PW_MAX_INPUTS), ("in_mod", ctypes.c_int64 * PW_MAX_INPUTS)]
 
 
+HEADS_CAUSAL, HEADS_ALIGN_END, HEADS_MAX_RUNS = 1, 2, 128
+
+
+class HeadsDesc(ctypes.Structure):
+    _fields_ = ([("dtype", ctypes.c_int32), ("flags", ctypes.c_int32)]
+                + [(n, ctypes.c_int64) for n in ("batch", "heads", "kv_heads", "seq_q", "seq_k", "d")]
+                + [(f"{n}_stride", ctypes.c_int64 * 3) for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv")]
+                + [("bias_stride", ctypes.c_int64 * 2), ("scale", ctypes.c_float), ("bias_dtype", ctypes.c_int32), ("buckets", ctypes.c_int32),
+                   ("n_runs", ctypes.c_int32), ("run_first", ctypes.c_int32 * HEADS_MAX_RUNS), ("run_bucket", ctypes.c_int32 * HEADS_MAX_RUNS)])
+
+
 EPI_NONE, EPI_GELU_TANH, EPI_RELU = 0, 1, 2
 EPILOGUES = {None: EPI_NONE, "none": EPI_NONE, "gelu_tanh": EPI_GELU_TANH, "relu": EPI_RELU}
 GEMM_B_NK = 1
@@ -113,6 +126,10 @@ _SIGNATURES = {
                                                         ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, ctypes.c_int64,
                                                         ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_float,
                                                         ctypes.c_void_p]),
+    "emmyb200_relative_runs": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32)]),
+    "emmyb200_attention_heads_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(HeadsDesc), ctypes.c_int]),
+    "emmyb200_attention_heads_fwd": (ctypes.c_int, [ctypes.POINTER(HeadsDesc)] + [ctypes.c_void_p] * 8 + [ctypes.c_int64, ctypes.c_void_p]),
+    "emmyb200_attention_heads_bwd": (ctypes.c_int, [ctypes.POINTER(HeadsDesc)] + [ctypes.c_void_p] * 13 + [ctypes.c_int64, ctypes.c_void_p]),
     "emmyb200_rowwise_workspace_bytes": (ctypes.c_int64, [ctypes.c_int, ctypes.c_int64, ctypes.c_int64]),
     "emmyb200_rowwise_f32": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                             ctypes.c_int64, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_int64,
@@ -596,6 +613,164 @@ def attention_allgather(q, k, v, dst_ptrs: list[int], scale: float | None = None
     check(library().emmyb200_attention_fwd_allgather(dtype_code(q), (ATT_CAUSAL if causal else 0) | (ATT_DST_MULTICAST if multicast else 0) | ATT_FORMS[form],
                                                      q.data_ptr(), k.data_ptr(), v.data_ptr(), arr, len(dst_ptrs),
                                                      units, q.shape[-2], k.shape[-2], d, scale, _stream(stream)))
+
+
+@functools.lru_cache(maxsize=64)
+def _relative_runs(buckets: int, max_distance: int, bidirectional: bool):
+    first, bucket = (ctypes.c_int32 * HEADS_MAX_RUNS)(), (ctypes.c_int32 * HEADS_MAX_RUNS)()
+    n = library().emmyb200_relative_runs(buckets, max_distance, 1 if bidirectional else 0, first, bucket)
+    if n < 0:
+        check(n)
+    return n, first, bucket
+
+
+def relative_runs(buckets: int, max_distance: int = 128, bidirectional: bool = True) -> list[tuple[int, int]]:
+    """The bucket scheme of the relative position bias as [(first distance, bucket), ...] in rising order of the distance
+    key position - query position; the first run reaches down without end."""
+    n, first, bucket = _relative_runs(int(buckets), int(max_distance), bool(bidirectional))
+    return [(first[i], bucket[i]) for i in range(n)]
+
+
+@functools.lru_cache(maxsize=512)
+def _heads_desc(backward: bool, dtype: int, flags: int, q_shape, k_shape, strides, scale: float, bias):
+    """The C description of a call and its workspace bytes, by sizes alone (`bias`: dtype, strides, buckets, max_distance, bidirectional)."""
+    desc = HeadsDesc()
+    desc.dtype, desc.flags, desc.scale = dtype, flags, scale
+    desc.batch, desc.heads, desc.seq_q, desc.d = q_shape
+    desc.kv_heads, desc.seq_k = k_shape[1], k_shape[2]
+    for name, stride in zip(("q", "k", "v", "o", "do", "dq", "dk", "dv"), strides):
+        getattr(desc, f"{name}_stride")[:] = stride
+    if bias is not None:
+        desc.bias_dtype, desc.bias_stride[:], desc.buckets = bias[0], bias[1], bias[2]
+        desc.n_runs, desc.run_first, desc.run_bucket = _relative_runs(*bias[2:])
+    need = library().emmyb200_attention_heads_workspace_bytes(ctypes.byref(desc), 1 if backward else 0)
+    if need < 0:
+        raise KernelError(-1, library().emmyb200_last_error().decode())
+    return desc, need
+
+
+def _heads_call(who: str, q, k, v, key_lens, bias_table, same_as_q: dict, same_as_k: dict):
+    """Checks what both directions share: shapes, one dtype and device, contiguous head dims."""
+    import torch
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"{who}: q is [batch, heads, seq_q, d], k and v [batch, kv_heads, seq_k, d]")
+    if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"{who}: shapes do not agree: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"{who}: float32, float16 or bfloat16")
+    for name, t, shape in [("q", q, q.shape), ("k", k, k.shape), ("v", v, k.shape), *((n, t, q.shape) for n, t in same_as_q.items()),
+                           *((n, t, k.shape) for n, t in same_as_k.items())]:
+        if not t.is_cuda:
+            raise RuntimeError("emmyb200 kernels take CUDA tensors only (there is no CPU path)")
+        if t.shape != shape or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"{who}: {name} is {tuple(t.shape)} {t.dtype} on {t.device}; wanted {tuple(shape)} {q.dtype} on {q.device}")
+        if t.stride(3) != 1:
+            raise ValueError(f"{who}: the head dim of {name} must be contiguous")
+    if key_lens is not None and (key_lens.dtype != torch.int32 or key_lens.shape != q.shape[:1] or key_lens.device != q.device or not key_lens.is_contiguous()):
+        raise ValueError(f"{who}: key_lens is a contiguous int32 vector [batch] on {q.device}")
+    if bias_table is not None and (bias_table.dim() != 2 or bias_table.shape[1] != q.shape[1] or bias_table.device != q.device
+                                   or bias_table.dtype not in (torch.float32, torch.float16, torch.bfloat16)):
+        raise ValueError(f"{who}: bias_table is a float [buckets, heads] tensor on {q.device}")
+
+
+def _heads_flags(who: str, causal: bool, align: str) -> int:
+    if align not in ("start", "end"):
+        raise ValueError(f"{who}: align is 'start' or 'end'")
+    return (HEADS_CAUSAL if causal else 0) | (HEADS_ALIGN_END if align == "end" else 0)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+@contextlib.contextmanager
+def _on(device, stream):
+    """The tensors' device and the launch's stream made current: what is allocated inside belongs to that stream."""
+    import torch
+    with torch.cuda.device(device):
+        if stream is None:
+            yield torch.cuda.current_stream().cuda_stream
+        else:
+            with torch.cuda.stream(stream):
+                yield stream.cuda_stream
+
+
+def _heads_workspace(who: str, workspace, need: int, device):
+    import torch
+    if need == 0:
+        return None
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous() or workspace.numel() < need:
+        raise ValueError(f"{who}: workspace is a contiguous uint8 tensor of at least {need} elements on {device}")
+    return workspace
+
+
+def attention_heads(q, k, v, scale: float | None = None, causal: bool = False, align: str = "start", key_lens=None, bias_table=None,
+                    max_distance: int = 128, bidirectional: bool = True, out=None, lse=None, workspace=None, stream=None):
+    """Attention over grouped heads: (o, lse) with o = softmax(q k^T * scale + bias) v and lse the float32 log-sum-exp of every
+    row, which `attention_heads_backward` needs.
+
+    q: [batch, heads, seq_q, d]; k, v: [batch, kv_heads, seq_k, d], heads a multiple of kv_heads; any strides with a
+    contiguous head dim (a transposed [batch, seq, heads, d] projection is taken as it is). `align`: query i stands at key
+    position i ("start") or at n - seq_q + i ("end": the queries are the last rows of the n keys, e.g. one token against a
+    cache). `causal`: a query sees keys up to its own position. `key_lens`: int32 [batch], the keys of each batch entry that
+    are seen (the rows behind them are never read). `bias_table`: [buckets, heads], added to the scores at
+    bucket(key position - query position), the buckets as `relative_runs(buckets, max_distance, bidirectional)`. A row that
+    sees no key gives o = 0 and lse = -inf."""
+    import torch
+    same = {} if out is None else {"out": out}
+    _heads_call("attention_heads", q, k, v, key_lens, bias_table, same, {})
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:3] or lse.device != q.device or not lse.is_contiguous()):
+        raise ValueError("attention_heads: lse is a contiguous float32 [batch, heads, seq_q] tensor")
+    with _on(q.device, stream) as handle:
+        out = torch.empty_like(q) if out is None else out
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if lse is None else lse
+        desc, need = _heads_desc(False, dtype_code(q), _heads_flags("attention_heads", causal, align), tuple(q.shape), tuple(k.shape),
+                                 tuple(t.stride()[:3] for t in (q, k, v, out)), q.shape[3] ** -0.5 if scale is None else float(scale),
+                                 _heads_bias(bias_table, max_distance, bidirectional))
+        workspace = _heads_workspace("attention_heads", workspace, need, q.device)
+        check(library().emmyb200_attention_heads_fwd(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lens), _ptr(bias_table),
+                                                     out.data_ptr(), lse.data_ptr(), _ptr(workspace), need, handle))
+    return out, lse
+
+
+def _heads_bias(table, max_distance: int, bidirectional: bool):
+    if table is None:
+        return None
+    return dtype_code(table), tuple(table.stride()), table.shape[0], int(max_distance), bool(bidirectional)
+
+
+def attention_heads_backward(do, q, k, v, o, lse, scale: float | None = None, causal: bool = False, align: str = "start", key_lens=None,
+                             bias_table=None, max_distance: int = 128, bidirectional: bool = True, dq=None, dk=None, dv=None, dtable=None,
+                             workspace=None, stream=None):
+    """Gradients (dq, dk, dv) -- with `bias_table` (dq, dk, dv, dtable) -- of `attention_heads` called with the same
+    arguments: `do` is the gradient of o; o and lse are what the forward gave. The probabilities are recomputed from
+    lse. The gradients of shared key heads are summed over their query heads, dtable over the batch; gradients of keys
+    behind key_lens are zero. Results do not depend on the order in which the blocks run."""
+    import torch
+    who = "attention_heads_backward"
+    _heads_call(who, q, k, v, key_lens, bias_table, {"do": do, "o": o, **({} if dq is None else {"dq": dq})},
+                {n: t for n, t in (("dk", dk), ("dv", dv)) if t is not None})
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:3] or lse.device != q.device or not lse.is_contiguous():
+        raise ValueError(f"{who}: lse is the contiguous float32 [batch, heads, seq_q] tensor of the forward")
+    if dtable is not None and (bias_table is None or dtable.shape != bias_table.shape or dtable.dtype != bias_table.dtype or dtable.device != q.device
+                               or not dtable.is_contiguous()):
+        raise ValueError(f"{who}: dtable is a contiguous tensor like bias_table")
+    with _on(q.device, stream) as handle:
+        dq = torch.empty_like(q) if dq is None else dq
+        dk = torch.empty_like(k) if dk is None else dk
+        dv = torch.empty_like(v) if dv is None else dv
+        if bias_table is not None and dtable is None:
+            dtable = torch.empty(bias_table.shape, dtype=bias_table.dtype, device=q.device)
+        desc, need = _heads_desc(True, dtype_code(q), _heads_flags(who, causal, align), tuple(q.shape), tuple(k.shape),
+                                 tuple(t.stride()[:3] for t in (q, k, v, o, do, dq, dk, dv)), q.shape[3] ** -0.5 if scale is None else float(scale),
+                                 _heads_bias(bias_table, max_distance, bidirectional))
+        workspace = _heads_workspace(who, workspace, need, q.device)
+        check(library().emmyb200_attention_heads_bwd(ctypes.byref(desc), do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+                                                     _ptr(key_lens), _ptr(bias_table), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable),
+                                                     _ptr(workspace), need, handle))
+    return (dq, dk, dv) if bias_table is None else (dq, dk, dv, dtable)
 
 
 def rowwise(op: str, x, weight=None, bias=None, eps: float = 0.0, out=None, workspace=None, stream=None):

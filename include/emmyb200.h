@@ -295,6 +295,66 @@ int emmyb200_attention_fwd_allgather(int dtype, int flags, const void* Q, const 
                                      void* const* O_dst, int n_dst, int64_t units, int64_t seq_q,
                                      int64_t seq_k, int64_t d, float scale, void* cuda_stream);
 
+/* Attention over heads, for training and serving: what emmyb200_attention_fwd computes, on strided buffers with grouped
+ * heads, a key count per batch entry, causal masks from either end and a learned relative position bias, keeping every
+ * row's log-sum-exp -- and its backward pass, which recomputes the probabilities from it. The reference is forward only
+ * and has equal heads; these entry points have no counterpart in it.
+ *
+ *   Q, O: [batch, heads, seq_q, d], K, V: [batch, kv_heads, seq_k, d], each with element strides of batch entries, heads
+ *   and rows (the head dim is contiguous; a projection's [batch, row, head, d] output is a choice of strides). heads is a
+ *   multiple of kv_heads: query head h reads key head h / (heads / kv_heads). lse: float[batch][heads][seq_q].
+ *   n_b = key_lens[b] keys are seen in batch entry b (device int32[batch], clamped to [0, seq_k]; NULL: seq_k), the rows
+ *   of K and V behind them are never read. Query i stands at key position pos = i, or n_b - seq_q + i with
+ *   EMMYB200_HEADS_ALIGN_END (the queries are the last rows of the keys: one token against a cache, a chunk of a prompt);
+ *   with EMMYB200_HEADS_CAUSAL it sees keys 0 .. pos.
+ *     s_ij = scale q_i . k_j + table[bucket(j - pos_i)][h],  lse_i = log sum_j exp s_ij,  o_i = sum_j exp(s_ij - lse_i) v_j
+ *   A row that sees no key gets o = 0, lse = -inf and zero gradients. fp32 scores, softmax and accumulation; one
+ *   rounding of each output. dtype F16 / BF16 with d = 64 or 128, 16-byte aligned buffers and strides that are multiples
+ *   of 8 run on the tensor cores (probabilities and their gradients are rounded to the dtype for the second products);
+ *   F32, d = 32 or 96, and other alignments run in fp32 arithmetic on the CUDA cores.
+ *
+ * The bias: `table` holds one value per bucket and head (bias_dtype, element strides bias_stride = {bucket, head}). The
+ * distance j - pos is mapped to its bucket by runs of rising distance: run r covers run_first[r] <= distance <
+ * run_first[r + 1] (run 0 reaches down, the last run up, without end; run_first[0] is not looked at) and belongs to bucket
+ * run_bucket[r]. emmyb200_relative_runs fills them for the usual scheme: with m buckets per direction (`buckets`, or half
+ * of them when bidirectional: the upper half for distance > 0), e = m / 2 and n = |distance| (one-sided: n =
+ * max(-distance, 0)), the bucket is n below e, else min(m - 1, e + floor(log(n / e) / log(max_distance / e) * (m - e))),
+ * the borders in exact arithmetic. It returns the number of runs, or a negative status. A table entry of -1e30 or less
+ * (-inf, the lowest value of a type) masks its pairs. n_runs = 0: no bias.
+ *
+ * Backward: from dO, the forward's inputs, O and lse,
+ *     p_ij = exp(s_ij - lse_i), D_i = dO_i . O_i, dS_ij = p_ij (dO_i . v_j - D_i)
+ *     dV_j = sum p_ij dO_i,  dK_j = scale sum dS_ij q_i (over the query heads of the key head),  dQ_i = scale sum dS_ij k_j
+ *     dtable[bucket][h] = sum of dS_ij over the batch and the pairs of that bucket
+ * dtable: [buckets][heads] contiguous, bias_dtype, NULL when not wanted. All gradients are overwritten, those of keys
+ * behind key_lens with zeros. No atomics on values: results do not depend on the order in which blocks finish.
+ *
+ * Workspace: emmyb200_attention_heads_workspace_bytes(desc, backward) bytes (0: none) of 256-byte aligned device memory,
+ * contents irrelevant before, undefined after; -1 for a description the call would reject. Calls that may run at the same time
+ * need workspaces of their own. */
+#define EMMYB200_HEADS_CAUSAL 1
+#define EMMYB200_HEADS_ALIGN_END 2
+#define EMMYB200_HEADS_MAX_RUNS 128
+typedef struct {
+    int32_t dtype, flags;
+    int64_t batch, heads, kv_heads, seq_q, seq_k, d;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];             /* elements: batch entry, head, row */
+    int64_t do_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];         /* backward only */
+    int64_t bias_stride[2];                                                 /* elements: bucket, head */
+    float scale;                                                            /* > 0 */
+    int32_t bias_dtype, buckets, n_runs;
+    int32_t run_first[EMMYB200_HEADS_MAX_RUNS], run_bucket[EMMYB200_HEADS_MAX_RUNS];
+} emmyb200_attention_heads_desc;
+int emmyb200_relative_runs(int buckets, int64_t max_distance, int bidirectional, int32_t* run_first, int32_t* run_bucket);
+int64_t emmyb200_attention_heads_workspace_bytes(const emmyb200_attention_heads_desc* desc, int backward);
+int emmyb200_attention_heads_fwd(const emmyb200_attention_heads_desc* desc, const void* Q, const void* K, const void* V,
+                                 const int32_t* key_lens, const void* table, void* O, float* lse, void* workspace,
+                                 int64_t workspace_bytes, void* cuda_stream);
+int emmyb200_attention_heads_bwd(const emmyb200_attention_heads_desc* desc, const void* dO, const void* Q, const void* K,
+                                 const void* V, const void* O, const float* lse, const int32_t* key_lens, const void* table,
+                                 void* dQ, void* dK, void* dV, void* dtable, void* workspace, int64_t workspace_bytes,
+                                 void* cuda_stream);
+
 /* Reductions over the last axis of a contiguous fp32 [rows, cols] array and the normalisations built on them:
  * the kernels the reference assembles from per-thread `Accum` loops, `WarpShuffle` butterflies and `TreeHalve`
  * shared-memory trees (emmyptx/kernel.py:786-797, :856-900) for the cases of tools/torch_cases/reductions.py:6-19
