@@ -31,6 +31,8 @@ uint64_t wait_limit_ns() { return g_wait_limit_ns.load(std::memory_order_relaxed
 // Implemented next to the kernels that own a status word.
 int gemm_read_status(uint32_t* out);
 int attention_read_status(uint32_t* out);
+int heads_fwd_read_status(uint32_t* out);
+int heads_bwd_read_status(uint32_t* out);
 
 }  // namespace emmy
 
@@ -46,10 +48,16 @@ extern "C" int emmyb200_device_status(uint32_t* status_out) {
     if (rc != EMMYB200_OK) return rc;
     rc = attention_read_status(&b);
     if (rc != EMMYB200_OK) return rc;
-    *status_out = a ? a : b;
+    uint32_t h = 0;
+    rc = heads_fwd_read_status(&h);
+    if (rc != EMMYB200_OK) return rc;
+    uint32_t g = 0;
+    rc = heads_bwd_read_status(&g);
+    if (rc != EMMYB200_OK) return rc;
+    *status_out = a ? a : b ? b : h ? h : g;
     if (*status_out != 0) {
         const uint32_t w = *status_out;
-        const char* kernel = (w >> 24) == 1 ? "gemm" : ((w >> 24) == 2 ? "attention" : ((w >> 24) == 0x7e ? "wait self-test" : "unknown"));
+        const char* kernel = (w >> 24) == 1 ? "gemm" : ((w >> 24) == 2 || (w >> 24) == 3 ? "attention" : ((w >> 24) >= 4 && (w >> 24) <= 6) ? "attention over heads" : ((w >> 24) == 0x7e ? "wait self-test" : "unknown"));
         return fail(EMMYB200_ERR_TIMEOUT, "a bounded device-side wait expired: status 0x%08x (%s kernel, wait site %u, stage %u)", w, kernel,
                     (w >> 16) & 0xffu, w & 0xffffu);
     }

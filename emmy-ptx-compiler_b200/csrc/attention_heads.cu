@@ -10,33 +10,60 @@ namespace emmy {
 int check_sm100();
 
 // ---- before the backward pass -------------------------------------------------------------------------------------------
-// One warp per row of the padded row arrays: delta = dO . O and lse2 = lse * log2(e). Rows behind seq_q and rows that saw
-// nothing get lse2 = +inf, which makes their probabilities 2^(s - inf) = 0 without a test in the kernels.
-template <typename T>
-__global__ void __launch_bounds__(256) heads_rows_kernel(HeadsParams p, HeadsGrads g, int d) {
+// One warp per row of the padded row arrays: -D = -dO . O and -lse * log2(e) + shift. Rows behind seq_q and rows that saw
+// nothing get -inf, which makes their probabilities 2^(s - inf) = 0 without a test in the kernels. NORMS (f16 on the tensor
+// cores): also the largest squared row norms of dO and of V per key head; a maximum does not depend on the order it is taken in.
+template <typename T, bool NORMS>
+__global__ void __launch_bounds__(256) heads_rows_kernel(HeadsParams p, HeadsGrads g, int d, float shift) {
     const int lane = threadIdx.x & 31;
-    const int64_t row_at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    int64_t row_at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int64_t rows = (int64_t)p.batch * p.heads * g.pad_q;
-    if (row_at >= rows) return;
-    const int row = (int)(row_at % g.pad_q);
-    const int64_t bh = row_at / g.pad_q;
-    const int b = (int)(bh / p.heads), h = (int)(bh % p.heads);
-    float sum = 0.0f;
-    if (row < p.seq_q) {
-        const T* o = static_cast<const T*>(g.o) + b * p.o_s[0] + h * p.o_s[1] + row * p.o_s[2];
-        const T* d_o = static_cast<const T*>(g.d_o) + b * p.do_s[0] + h * p.do_s[1] + row * p.do_s[2];
-        for (int c = lane; c < d; c += 32) sum = fmaf(heads_load(o, c), heads_load(d_o, c), sum);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (lane == 0) {
-        float l = INFINITY;
+    float sum = 0.0f, norm = 0.0f;
+    int64_t bk = -1;
+    if (row_at < rows) {
+        const int row = (int)(row_at % g.pad_q);
+        const int64_t bh = row_at / g.pad_q;
+        const int b = (int)(bh / p.heads), h = (int)(bh % p.heads);
         if (row < p.seq_q) {
-            const float v = g.lse[bh * p.seq_q + row];
-            l = v == -INFINITY ? INFINITY : v * kLog2e;
+            const T* o = static_cast<const T*>(g.o) + b * p.o_s[0] + h * p.o_s[1] + row * p.o_s[2];
+            const T* d_o = static_cast<const T*>(g.d_o) + b * p.do_s[0] + h * p.do_s[1] + row * p.do_s[2];
+            for (int c = lane; c < d; c += 32) {
+                const float v = heads_load(d_o, c);
+                sum = fmaf(heads_load(o, c), v, sum);
+                if (NORMS) norm = fmaf(v, v, norm);
+            }
         }
-        g.lse2[row_at] = l;
-        g.delta[row_at] = sum;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (lane == 0) {
+            float l = -INFINITY;
+            if (row < p.seq_q) {
+                const float v = g.lse[bh * p.seq_q + row];
+                l = v == -INFINITY ? -INFINITY : fmaf(v, -kLog2e, shift);
+            }
+            g.lse2[row_at] = l;
+            g.delta[row_at] = -sum;
+        }
+        bk = (int64_t)b * p.kv_heads + h / p.group;
+    } else if (NORMS) {
+        row_at -= rows;
+        bk = row_at / p.seq_k;
+        const int row = (int)(row_at % p.seq_k);
+        if (bk < (int64_t)p.batch * p.kv_heads) {
+            const int b = (int)(bk / p.kv_heads);
+            if (row < heads_key_count(p, b)) {
+                const T* v = static_cast<const T*>(g.v) + b * p.v_s[0] + (bk % p.kv_heads) * p.v_s[1] + row * p.v_s[2];
+                for (int c = lane; c < d; c += 32) norm = fmaf(heads_load(v, c), heads_load(v, c), norm);
+            }
+            bk += (int64_t)p.batch * p.kv_heads;
+        } else {
+            bk = -1;
+        }
+    }
+    if (NORMS && bk >= 0) {                     // non-negative floats order as their bit patterns; NaN above all
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, off);
+        if (lane == 0) atomicMax(reinterpret_cast<unsigned int*>(g.amax) + bk, __float_as_uint(norm));
     }
 }
 
@@ -141,19 +168,20 @@ static HeadsParams make_params(const emmyb200_attention_heads_desc* c, const int
     return p;
 }
 
-// Workspace of a backward pass: [lse2][delta][run sums], each 256-byte aligned.
+// Workspace of a backward pass: [lse2][delta][run sums][amax], each 256-byte aligned. Large enough for either kind of kernels.
 struct BwdLayout {
-    int64_t pad_q, q_tiles, delta_at, sums_at, total;
+    int64_t pad_q, parts, delta_at, sums_at, amax_at, total;
 };
 static int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 static BwdLayout bwd_layout(const emmyb200_attention_heads_desc* c) {
     BwdLayout w;
     w.pad_q = (c->seq_q + 127) / 128 * 128;
-    w.q_tiles = (c->seq_q + kCoresTile - 1) / kCoresTile;
+    w.parts = w.pad_q / 128 * 8;                // tensor cores: eight warps per 128 queries; CUDA cores: one part per 64
     const int64_t rows = round256(c->batch * c->heads * w.pad_q * 4);
     w.delta_at = rows;
     w.sums_at = 2 * rows;
-    w.total = w.sums_at + round256(c->n_runs ? c->batch * c->heads * w.q_tiles * c->n_runs * 4 : 0);
+    w.amax_at = w.sums_at + round256(c->n_runs ? c->batch * c->heads * w.parts * c->n_runs * 4 : 0);
+    w.total = w.amax_at + (c->dtype == EMMYB200_F16 ? round256(2 * c->batch * c->kv_heads * 4) : 0);
     return w;
 }
 
@@ -195,7 +223,9 @@ extern "C" int emmyb200_relative_runs(int buckets, int64_t max_distance, int bid
 extern "C" int64_t emmyb200_attention_heads_workspace_bytes(const emmyb200_attention_heads_desc* c, int backward) {
     using namespace emmy;
     if (check_desc(c, backward != 0, "attention_heads_workspace_bytes") != EMMYB200_OK) return -1;
-    return backward ? bwd_layout(c).total : 0;
+    if (backward) return bwd_layout(c).total;
+    if (c->batch * c->heads * c->seq_q * c->seq_k == 0 || c->dtype == EMMYB200_F32 || (c->d != 64 && c->d != 128)) return 0;
+    return fwd_workspace(heads_fwd_plan(make_params(c, nullptr, nullptr)), c->d);
 }
 
 extern "C" int emmyb200_attention_heads_fwd(const emmyb200_attention_heads_desc* c, const void* Q, const void* K, const void* V,
@@ -212,7 +242,10 @@ extern "C" int emmyb200_attention_heads_fwd(const emmyb200_attention_heads_desc*
         return fail(EMMYB200_ERR_ARG, "attention_heads_fwd: needs %lld bytes of 256-byte aligned workspace", (long long)need);
     rc = check_sm100();
     if (rc != EMMYB200_OK) return rc;
-    return heads_fwd_cores(c->dtype, (int)c->d, make_params(c, key_lens, table), Q, K, V, O, lse, static_cast<cudaStream_t>(cuda_stream));
+    const HeadsParams p = make_params(c, key_lens, table);
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    if (heads_sm100_takes(p, c->dtype, (int)c->d, Q, K, V, O)) return heads_fwd_sm100(c->dtype, (int)c->d, p, heads_fwd_plan(p), Q, K, V, O, lse, workspace, s);
+    return heads_fwd_cores(c->dtype, (int)c->d, p, Q, K, V, O, lse, s);
 }
 
 extern "C" int emmyb200_attention_heads_bwd(const emmyb200_attention_heads_desc* c, const void* dO, const void* Q, const void* K,
@@ -238,21 +271,28 @@ extern "C" int emmyb200_attention_heads_bwd(const emmyb200_attention_heads_desc*
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     HeadsGrads g = {};
     g.d_o = dO; g.q = Q; g.k = K; g.v = V; g.o = O; g.lse = lse; g.dq = dQ; g.dk = dK; g.dv = dV; g.dtable = dtable;
-    g.pad_q = (int)w.pad_q; g.q_tiles = (int)w.q_tiles;
+    g.pad_q = (int)w.pad_q;
     g.lse2 = reinterpret_cast<float*>(ws);
     g.delta = reinterpret_cast<float*>(ws + w.delta_at);
     g.run_sums = reinterpret_cast<float*>(ws + w.sums_at);
+    g.amax = reinterpret_cast<float*>(ws + w.amax_at);
+    const bool tensor_cores = has_q && has_k && heads_bwd_sm100_takes(p, c->dtype, (int)c->d, g);
+    const bool norms = tensor_cores && c->dtype == EMMYB200_F16;
+    g.q_tiles = (int)(tensor_cores ? w.parts : (c->seq_q + kCoresTile - 1) / kCoresTile);
     if (has_q) {
-        const int64_t blocks = (c->batch * c->heads * w.pad_q + 7) / 8;
+        const int64_t blocks = (c->batch * c->heads * w.pad_q + (norms ? c->batch * c->kv_heads * c->seq_k : 0) + 7) / 8;
         if (blocks >= (1ll << 31)) return fail(EMMYB200_ERR_SHAPE, "attention_heads_bwd: %lld rows exceed the grid limit", (long long)blocks * 8);
-        if (c->dtype == EMMYB200_F32) heads_rows_kernel<float><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d);
-        else if (c->dtype == EMMYB200_F16) heads_rows_kernel<__half><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d);
-        else heads_rows_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d);
+        const float shift = tensor_cores ? heads_bwd_shift(c->dtype) : 0.0f;
+        if (norms) EMMY_CUDA(cudaMemsetAsync(g.amax, 0, 2 * c->batch * c->kv_heads * 4, s));
+        if (norms) heads_rows_kernel<__half, true><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d, shift);
+        else if (c->dtype == EMMYB200_F32) heads_rows_kernel<float, false><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d, shift);
+        else if (c->dtype == EMMYB200_F16) heads_rows_kernel<__half, false><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d, shift);
+        else heads_rows_kernel<__nv_bfloat16, false><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d, shift);
         rc = launch_status("heads_rows_kernel");
         if (rc != EMMYB200_OK) return rc;
     }
     if (has_q || has_k) {
-        rc = heads_bwd_cores(c->dtype, (int)c->d, p, g, s);
+        rc = tensor_cores ? heads_bwd_sm100(c->dtype, (int)c->d, p, g, s) : heads_bwd_cores(c->dtype, (int)c->d, p, g, s);
         if (rc != EMMYB200_OK) return rc;
     }
     if (dtable != nullptr && c->heads > 0) {

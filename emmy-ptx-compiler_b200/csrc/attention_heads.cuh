@@ -35,10 +35,11 @@ struct HeadsGrads {
     const float* lse;
     void *dq, *dk, *dv, *dtable;
     int pad_q;                  // rows per (batch entry, head) of lse2 and delta: seq_q rounded up to 128
-    float* lse2;                // lse * log2(e); +inf for rows that see nothing and rows behind seq_q: their probabilities come out 0
-    float* delta;               // D_i = dO_i . O_i
-    float* run_sums;            // [batch][heads][query tiles][n_runs]: sums of dS by run, added up in order by the last kernel
-    int q_tiles;                // of run_sums
+    float* lse2;                // -lse * log2(e) + a shift (0 on the CUDA cores); -inf for rows that see nothing and rows behind seq_q:
+                                // their probabilities 2^(s + lse2) come out 0
+    float* delta;               // -D_i = -dO_i . O_i
+    float* run_sums;            // [batch][heads][q_tiles][n_runs]: sums of dS by run, added up in order by the last kernel
+    int q_tiles;                // parts a (batch entry, head) is summed in
     float* amax;                // f16 tensor-core path: [2][batch * kv_heads] largest row norms (squared) of dO and V
 };
 
@@ -83,5 +84,21 @@ __device__ __forceinline__ int heads_run_of(const int* first, int n_runs, int di
 int heads_fwd_cores(int dtype, int d, const HeadsParams& p, const void* Q, const void* K, const void* V, void* O, float* lse, cudaStream_t s);
 int heads_bwd_cores(int dtype, int d, const HeadsParams& p, const HeadsGrads& g, cudaStream_t s);
 constexpr int kCoresTile = 64;                  // query and key tile of the CUDA-core kernels
+
+// Tensor cores: 16-bit operands with d = 64 or 128 that TMA can address (heads_sm100_takes).
+struct FwdPlan {
+    int packed, tiles, splits;                  // see attention_heads_fwd_sm100.cu
+    int64_t rows;                               // batch * heads * seq_q
+};
+FwdPlan heads_fwd_plan(const HeadsParams& p);
+// Workspace of split keys: float2[splits][rows], then float[splits][rows][d].
+inline int64_t fwd_part_offset(const FwdPlan& w) { return (w.splits * w.rows * 8 + 255) / 256 * 256; }
+inline int64_t fwd_workspace(const FwdPlan& w, int64_t d) { return w.splits == 1 ? 0 : (fwd_part_offset(w) + w.splits * w.rows * d * 4 + 255) / 256 * 256; }
+bool heads_sm100_takes(const HeadsParams& p, int dtype, int d, const void* Q, const void* K, const void* V, const void* O);
+int heads_fwd_sm100(int dtype, int d, const HeadsParams& p, const FwdPlan& plan, const void* Q, const void* K, const void* V, void* O, float* lse,
+                    void* workspace, cudaStream_t s);
+bool heads_bwd_sm100_takes(const HeadsParams& p, int dtype, int d, const HeadsGrads& g);
+float heads_bwd_shift(int dtype);               // of lse2
+int heads_bwd_sm100(int dtype, int d, const HeadsParams& p, const HeadsGrads& g, cudaStream_t s);
 
 }  // namespace emmy

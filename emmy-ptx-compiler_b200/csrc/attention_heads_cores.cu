@@ -235,9 +235,9 @@ __global__ void __launch_bounds__(kCThreads) heads_dkv_cores_kernel(HeadsParams 
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const float t = cores_score(p, cb, s[r][c], 4 * ty + r, tx + 16 * c, row0, key0, offset, n_keys);
-                        const float pr = exp2f(t - lse2);
+                        const float pr = exp2f(t + lse2);
                         p_s[(4 * ty + r) * kPRow + tx + 16 * c] = pr;
-                        ds_s[(4 * ty + r) * kPRow + tx + 16 * c] = pr * (dp[r][c] - delta);
+                        ds_s[(4 * ty + r) * kPRow + tx + 16 * c] = pr * (dp[r][c] + delta);
                     }
                 }
                 __syncthreads();
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kCThreads) heads_dq_cores_kernel(HeadsParams p
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const float t = cores_score(p, cb, s[r][c], 4 * ty + r, tx + 16 * c, row0, key0, offset, n_keys);
-                s[r][c] = exp2f(t - lse2[r]) * (dp[r][c] - delta[r]);
+                s[r][c] = exp2f(t + lse2[r]) * (dp[r][c] + delta[r]);
             }
 #pragma unroll
         for (int c = 0; c < 4; ++c)

@@ -1,0 +1,125 @@
+// Device pieces shared by the tensor-core kernels of attention over heads: packed fp32 arithmetic, rounding pairs to 16
+// bits, the relative position bias of a warp's block of scores, and the tensor maps of strided [batch, head, row, d]
+// operands.
+#pragma once
+#include <limits.h>
+
+#include "attention_heads.cuh"
+#include "sm100_ptx.cuh"
+
+namespace emmy {
+namespace heads {
+
+constexpr int kTile = 128;              // query rows and keys of a tile
+// bf16 operands are made by cutting the fp32 pattern (one byte permute per pair; a conversion would run on the
+// transcendental unit next to the exponentials). The cut loses half a step, 2^-8 of a value with mantissa 1, on average 2^-8 / ln 4 of
+// values spread evenly in magnitude: they are scaled by 1 + 2^-8 / ln 4 first, which leaves no mean error and at most 1.28 times the
+// 2^-8 of a rounding.
+constexpr float kCutScale = 1.0028178f;
+constexpr float kCutScaleLog2 = 0.0040594572f;      // its log2
+
+__device__ __forceinline__ uint64_t as_u64(float2 v) { return *reinterpret_cast<uint64_t*>(&v); }
+__device__ __forceinline__ float2 as_f2(uint64_t v) { return *reinterpret_cast<float2*>(&v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
+    return as_f2(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)));
+    return as_f2(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_u64(a)), "l"(as_u64(b)));
+    return as_f2(d);
+}
+__device__ __forceinline__ float2 f2(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
+
+// Nearest: outputs.
+template <bool BF16>
+__device__ __forceinline__ uint32_t round_pair(float lo, float hi) {
+    if constexpr (BF16) {
+        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&v);
+    } else {
+        __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&v);
+    }
+}
+// Operands of a second product: bf16 values already scaled by 1 + 2^-9 are cut, f16 ones rounded.
+template <bool BF16>
+__device__ __forceinline__ uint32_t operand_pair(float2 v) {
+    if constexpr (BF16) return __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
+    else return round_pair<false>(v.x, v.y);
+}
+
+// ---- the bias --------------------------------------------------------------------------------------------------------
+// A warp works on 32 x 64 blocks of scores, which span 95 distances. Where they all fall into one run (far from the
+// diagonal: every distance beyond max_distance) the bias is one number; else the warp looks the 95 up (a binary search
+// each, three a lane) into its own stretch of shared memory. The range of the run is kept, so that neighbouring
+// blocks of a far stretch cost two comparisons.
+struct BiasShared {
+    int first[kHeadsMaxRuns];
+    float value[kHeadsMaxRuns];         // of the head, log2 units
+    float by_dist[8][96];               // one row per warp
+};
+struct WarpBias {
+    int lo, hi;                         // distances [lo, hi) have the bias `same`
+    int run;                            // its run
+    float same;
+    __device__ __forceinline__ void reset() { lo = 0; hi = 0; run = 0; same = 0.0f; }
+    // Distances d0 .. d0 + 94. True: all in one run. False: s.by_dist[warp][0 .. 94] holds their biases. `value`: by run.
+    __device__ __forceinline__ bool block(BiasShared& s, const float* value, int warp, int lane, int n_runs, int d0) {
+        if (d0 >= lo && d0 + 94 < hi) return true;
+        int r[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) r[k] = heads_run_of(s.first, n_runs, d0 + 32 * k + lane);
+        const int ra = __shfl_sync(0xffffffffu, r[0], 0), rb = __shfl_sync(0xffffffffu, r[2], 30);
+        if (ra == rb) {
+            lo = ra == 0 ? INT_MIN : s.first[ra];
+            hi = ra + 1 == n_runs ? INT_MAX : s.first[ra + 1];
+            run = ra;
+            same = value[ra];
+            return true;
+        }
+        __syncwarp();                   // the previous block's readers
+#pragma unroll
+        for (int k = 0; k < 3; ++k) s.by_dist[warp][32 * k + lane] = value[r[k]];
+        __syncwarp();
+        return false;
+    }
+};
+__device__ __forceinline__ void load_bias(BiasShared& s, const HeadsParams& p, int head, int tid, int threads) {
+    for (int r = tid; r < p.n_runs; r += threads) {
+        s.first[r] = p.run_first[r];
+        s.value[r] = heads_run_bias(p, r, head);
+    }
+}
+
+// ---- strided operands ---------------------------------------------------------------------------------------------------
+// A [batch, heads, rows, d] operand as a 4-D tensor map; dimensions with stride 0 (a broadcast) or extent 1 are given
+// extent 1 and coordinate 0.
+struct MapAt {
+    int head, batch;                    // 1, or 0 where the coordinate is always 0
+};
+
+inline bool stride_fits(int64_t extent, int64_t s) { return extent <= 1 || s == 0 || (s % 8 == 0 && s < (1ll << 38)); }
+// Whether TMA can address the operand (16-byte aligned base, strides in whole 16-byte units).
+inline bool map_fits(const void* base, int64_t batch, int64_t heads, int64_t rows, const int64_t* s) {
+    return aligned(base, 16) && stride_fits(batch, s[0]) && stride_fits(heads, s[1]) && stride_fits(rows, s[2]) && !(rows > 1 && s[2] == 0);
+}
+inline int make_map(CUtensorMap* map, MapAt* at, const void* base, int64_t batch, int64_t heads, int64_t rows, int d, const int64_t* s, int box_rows,
+                    int box_heads) {
+    at->batch = batch > 1 && s[0] != 0;
+    at->head = heads > 1 && s[1] != 0;
+    const uint64_t row_s = rows > 1 ? (uint64_t)s[2] : (uint64_t)d;
+    const uint64_t extent[4] = {(uint64_t)d, (uint64_t)rows, at->head ? (uint64_t)heads : 1, at->batch ? (uint64_t)batch : 1};
+    const uint64_t stride[3] = {row_s, at->head ? (uint64_t)s[1] : row_s, at->batch ? (uint64_t)s[0] : row_s};
+    const uint32_t box[4] = {64, (uint32_t)box_rows, (uint32_t)box_heads, 1};
+    return make_tensor_map_4d(map, base, extent, stride, box);
+}
+
+}  // namespace heads
+}  // namespace emmy

@@ -445,6 +445,20 @@ int make_tensor_map_3d_strided(CUtensorMap* out, const void* base, uint64_t plan
     return EMMYB200_OK;
 }
 
+int make_tensor_map_4d(CUtensorMap* out, const void* base, const uint64_t (&extent)[4], const uint64_t (&stride)[3], const uint32_t (&box_extent)[4]) {
+    EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return fail(EMMYB200_ERR_DEVICE, "cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[4] = {extent[0], extent[1], extent[2], extent[3]};
+    cuuint64_t strides[3] = {stride[0] * 2, stride[1] * 2, stride[2] * 2};
+    cuuint32_t box[4] = {box_extent[0], box_extent[1], box_extent[2], box_extent[3]};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(EMMYB200_ERR_ARG, "cuTensorMapEncodeTiled (4-D) failed: %d", (int)r);
+    return EMMYB200_OK;
+}
+
 // The fp32 output of the split-precision GEMM: 32-column (128-byte) boxes.
 int make_tensor_map_3d_f32(CUtensorMap* out, const void* base, uint64_t planes, uint64_t rows, uint64_t cols, uint64_t ld,
                            uint64_t plane_stride, uint32_t box_rows, uint32_t box_cols) {

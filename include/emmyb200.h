@@ -427,7 +427,7 @@ int emmyb200_launch(const char* handle_json, void* const* params, int n_params, 
                     void* cuda_stream);
 
 /* Reads (and clears) the device status word of the current device into *status_out: 0 if no bounded wait has
- * expired since the last call, else a code naming kernel (bits 24-31: 1 GEMM, 2 attention), wait site (16-23)
+ * expired since the last call, else a code naming kernel (bits 24-31: 1 GEMM, 2 and 3 attention, 4 to 6 attention over heads), wait site (16-23)
  * and pipeline stage (0-15). Returns EMMYB200_OK with a zero word and EMMYB200_ERR_TIMEOUT with a non-zero one
  * (the outputs of the launches since the last clean read are then not to be trusted; the device and the library
  * stay usable). Synchronises the device. This replaces the reference's only device-side error path, a `trap`

@@ -10,9 +10,12 @@ probability in fp32 and |.| the same sums over absolute values:
     dtable:  u |dtable| + g sum p (|do|.|v| + |do|.|o|)
     lse:     g
 w is the rounding of a probability (or of its gradient) to 16 bits before the second product: 1.5 half steps where the tensor
-cores run (bf16 values are cut after scaling by 1 + 2^-9, off by at most 2^-7 - 2^-9), none in fp32 arithmetic. f16
+cores run (bf16 values are cut after scaling by 1 + 2^-8 / ln 4, off by at most 2^-7 less that: 1.28 half steps), none in fp32 arithmetic. f16
 probabilities below 2^-14 of the row's largest lose bits: 2^-24 sum |v| more in o. An f16 output below 2^-14 is off by up to
-2^-25, half a step there.
+2^-25, half a step there. The backward keeps p 2^14 and ds 2^14 g in f16, g the power of two at or below 1 / B with B = max |dO row| max
+|v row| of a key head; below 2^-14 those values are off by up to 2^-25 too, which is 2^-39 of p and 2^-39 / g <= 2^-38 B of ds: another
+2^-39 sum |do| in dv, scale 2^-38 B sum |k| in dq (|q| in dk), over the pairs that are seen. (A score range of hundreds, as in
+test_large_scores, has keys whose whole gradient is of that size.)
 """
 import math
 
@@ -90,6 +93,10 @@ class Case:
         r["dv_abs"] = shared(p.transpose(-1, -2) @ do.abs())
         for w, x in (("ds", ds.abs()), ("fp", ds_abs)):
             r[f"dq_{w}"], r[f"dk_{w}"] = x @ kx.abs() * self.scale, shared(x.transpose(-1, -2) @ q.abs()) * self.scale
+        once = torch.where(seen, 1.0, 0.0).double()
+        big = do.norm(dim=-1).amax() * vx.norm(dim=-1).amax() if do.numel() and vx.numel() else 0.0
+        r["dv_tiny"] = 2.0 ** -39 * shared(once.transpose(-1, -2) @ do.abs())
+        r["dq_tiny"], r["dk_tiny"] = 2.0 ** -38 * big * self.scale * (once @ kx.abs()), 2.0 ** -38 * big * self.scale * shared(once.transpose(-1, -2) @ q.abs())
         if self.table is not None:
             flat = bucket[:, None].expand_as(ds).transpose(0, 1).reshape(h, -1)
             r["dtable"] = torch.zeros(h, self.table.shape[0], dtype=torch.float64, device=q.device).scatter_add_(1, flat, ds.transpose(0, 1).reshape(h, -1)).t()
@@ -122,9 +129,10 @@ class Case:
         torch.cuda.synchronize()
         assert runtime.device_status() == 0
         assert len(grads) == (3 if self.table is None else 4)
-        self.check("dv", grads[2], r["dv"], u * r["dv"].abs() + (w + r["g"]) * r["dv_abs"])
-        self.check("dq", grads[0], r["dq"], u * r["dq"].abs() + w * r["dq_ds"] + r["g"] * r["dq_fp"])
-        self.check("dk", grads[1], r["dk"], u * r["dk"].abs() + w * r["dk_ds"] + r["g"] * r["dk_fp"])
+        f16 = 1.0 if tiny else 0.0
+        self.check("dv", grads[2], r["dv"], u * r["dv"].abs() + (w + r["g"]) * r["dv_abs"] + f16 * r["dv_tiny"])
+        self.check("dq", grads[0], r["dq"], u * r["dq"].abs() + w * r["dq_ds"] + r["g"] * r["dq_fp"] + f16 * r["dq_tiny"])
+        self.check("dk", grads[1], r["dk"], u * r["dk"].abs() + w * r["dk_ds"] + r["g"] * r["dk_fp"] + f16 * r["dk_tiny"])
         if self.table is not None:
             ut = torch.finfo(self.table.dtype).eps / 2
             self.check("dtable", grads[3], r["dtable"], ut * r["dtable"].abs() + r["g"] * r["dtable_abs"])
