@@ -10,61 +10,116 @@ namespace emmy {
 int check_sm100();
 
 // ---- before the backward pass -------------------------------------------------------------------------------------------
-// One warp per row of the padded row arrays: -D = -dO . O and -lse * log2(e) + shift. Rows behind seq_q and rows that saw
-// nothing get -inf, which makes their probabilities 2^(s - inf) = 0 without a test in the kernels. NORMS (f16 on the tensor
-// cores): also the largest squared row norms of dO and of V per key head; a maximum does not depend on the order it is taken in.
-template <typename T, bool NORMS>
-__global__ void __launch_bounds__(256) heads_rows_kernel(HeadsParams p, HeadsGrads g, int d, float shift) {
+// Row terms of the padded row arrays: -D = -dO . O and -lse * log2(e) + shift. Rows behind seq_q and rows that saw nothing get
+// -inf, which makes their probabilities 2^(s - inf) = 0 without a test in the kernels.
+__device__ __forceinline__ void store_row(const HeadsParams& p, const HeadsGrads& g, int64_t bh, int row, float dot, float shift) {
+    float l = -INFINITY;
+    if (row < p.seq_q) {
+        const float v = g.lse[bh * p.seq_q + row];
+        l = v == -INFINITY ? -INFINITY : fmaf(v, -kLog2e, shift);
+    }
+    g.lse2[bh * g.pad_q + row] = l;
+    g.delta[bh * g.pad_q + row] = -dot;
+}
+
+// Any type and alignment: one warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) heads_rows_kernel(HeadsParams p, HeadsGrads g, int d) {
     const int lane = threadIdx.x & 31;
-    int64_t row_at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t rows = (int64_t)p.batch * p.heads * g.pad_q;
-    float sum = 0.0f, norm = 0.0f;
-    int64_t bk = -1;
-    if (row_at < rows) {
-        const int row = (int)(row_at % g.pad_q);
-        const int64_t bh = row_at / g.pad_q;
-        const int b = (int)(bh / p.heads), h = (int)(bh % p.heads);
-        if (row < p.seq_q) {
-            const T* o = static_cast<const T*>(g.o) + b * p.o_s[0] + h * p.o_s[1] + row * p.o_s[2];
-            const T* d_o = static_cast<const T*>(g.d_o) + b * p.do_s[0] + h * p.do_s[1] + row * p.do_s[2];
-            for (int c = lane; c < d; c += 32) {
-                const float v = heads_load(d_o, c);
-                sum = fmaf(heads_load(o, c), v, sum);
-                if (NORMS) norm = fmaf(v, v, norm);
-            }
-        }
+    const int64_t row_at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row_at >= (int64_t)p.batch * p.heads * g.pad_q) return;
+    const int row = (int)(row_at % g.pad_q);
+    const int64_t bh = row_at / g.pad_q;
+    const int b = (int)(bh / p.heads), h = (int)(bh % p.heads);
+    float sum = 0.0f;
+    if (row < p.seq_q) {
+        const T* o = static_cast<const T*>(g.o) + b * p.o_s[0] + h * p.o_s[1] + row * p.o_s[2];
+        const T* d_o = static_cast<const T*>(g.d_o) + b * p.do_s[0] + h * p.do_s[1] + row * p.do_s[2];
+        for (int c = lane; c < d; c += 32) sum = fmaf(heads_load(o, c), heads_load(d_o, c), sum);
+    }
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (lane == 0) {
-            float l = -INFINITY;
-            if (row < p.seq_q) {
-                const float v = g.lse[bh * p.seq_q + row];
-                l = v == -INFINITY ? -INFINITY : fmaf(v, -kLog2e, shift);
-            }
-            g.lse2[row_at] = l;
-            g.delta[row_at] = -sum;
-        }
-        bk = (int64_t)b * p.kv_heads + h / p.group;
-    } else if (NORMS) {
-        row_at -= rows;
-        bk = row_at / p.seq_k;
-        const int row = (int)(row_at % p.seq_k);
-        if (bk < (int64_t)p.batch * p.kv_heads) {
-            const int b = (int)(bk / p.kv_heads);
-            if (row < heads_key_count(p, b)) {
-                const T* v = static_cast<const T*>(g.v) + b * p.v_s[0] + (bk % p.kv_heads) * p.v_s[1] + row * p.v_s[2];
-                for (int c = lane; c < d; c += 32) norm = fmaf(heads_load(v, c), heads_load(v, c), norm);
-            }
-            bk += (int64_t)p.batch * p.kv_heads;
-        } else {
-            bk = -1;
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == 0) store_row(p, g, bh, row, sum, 0.0f);
+}
+
+// 16-bit rows of 64 or 128 aligned elements, as the tensor-core kernels take them: bound by the bytes of dO and O. D / 8 lanes share a
+// row with one 128-bit access each, four rows per thread in flight (4 Mi rows of 128, bf16: see the table of measurements). A block's
+// rows belong to one (batch entry, head). f16 (NORMS): also the largest squared row norms of dO and, in the blocks behind
+// those, of V's rows below the key count; a maximum does not depend on the order it is taken in.
+template <typename T, int D, bool NORMS>
+__global__ void __launch_bounds__(256) heads_rows16_kernel(HeadsParams p, HeadsGrads g, float shift, int q_blocks) {
+    constexpr int kLanes = D / 8, kRowsPerPass = 256 / kLanes, kPasses = 4, kRows = kRowsPerPass * kPasses;     // 64 or 128 rows
+    const int sub = threadIdx.x % kLanes, first = threadIdx.x / kLanes;
+    const bool is_q = !NORMS || (int)blockIdx.x < q_blocks;
+    const int block = is_q ? blockIdx.x : blockIdx.x - q_blocks;
+    const int pad_k = (p.seq_k + 127) / 128 * 128, per = (is_q ? g.pad_q : pad_k) / kRows;
+    const int bh = block / per, row0 = block % per * kRows;
+    const int heads = is_q ? p.heads : p.kv_heads;
+    const int b = bh / heads, h = bh % heads;
+    const T* x = is_q ? static_cast<const T*>(g.d_o) + b * p.do_s[0] + h * p.do_s[1] : static_cast<const T*>(g.v) + b * p.v_s[0] + h * p.v_s[1];
+    const int64_t x_row = is_q ? p.do_s[2] : p.v_s[2];
+    const T* o = is_q ? static_cast<const T*>(g.o) + b * p.o_s[0] + h * p.o_s[1] : x;
+    const int64_t o_row = is_q ? p.o_s[2] : x_row;
+    const int rows = is_q ? p.seq_q : heads_key_count(p, b);
+    uint4 xv[kPasses], ov[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+        const int row = row0 + i * kRowsPerPass + first;
+        xv[i] = ov[i] = make_uint4(0, 0, 0, 0);
+        if (row < rows) {
+            xv[i] = __ldg(reinterpret_cast<const uint4*>(x + row * x_row) + sub);
+            if (is_q) ov[i] = __ldg(reinterpret_cast<const uint4*>(o + row * o_row) + sub);
         }
     }
-    if (NORMS && bk >= 0) {                     // non-negative floats order as their bit patterns; NaN above all
+    float most = 0.0f;
+    bool nan = false;
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, off);
-        if (lane == 0) atomicMax(reinterpret_cast<unsigned int*>(g.amax) + bk, __float_as_uint(norm));
+    for (int i = 0; i < kPasses; ++i) {
+        const T* xe = reinterpret_cast<const T*>(&xv[i]);
+        const T* oe = reinterpret_cast<const T*>(&ov[i]);
+        float dot = 0.0f, norm = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float v = heads_load(xe, k);
+            dot = fmaf(heads_load(oe, k), v, dot);
+            if (NORMS) norm = fmaf(v, v, norm);
+        }
+#pragma unroll
+        for (int off = kLanes / 2; off > 0; off >>= 1) {
+            dot += __shfl_xor_sync(0xffffffffu, dot, off);
+            if (NORMS) norm += __shfl_xor_sync(0xffffffffu, norm, off);
+        }
+        if (is_q && sub == 0) store_row(p, g, bh, row0 + i * kRowsPerPass + first, dot, shift);
+        if (NORMS) {
+            nan |= !(norm == norm);
+            most = fmaxf(most, norm);
+        }
     }
+    if (NORMS) {
+        if (nan) most = INFINITY;               // as for an infinite norm: no scaling
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+        __shared__ float warp_most[8];
+        if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = most;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) most = fmaxf(most, warp_most[k]);
+            const int64_t bk = is_q ? (int64_t)b * p.kv_heads + h / p.group : (int64_t)p.batch * p.kv_heads + bh;
+            atomicMax(reinterpret_cast<unsigned int*>(g.amax) + bk, __float_as_uint(most));        // not negative: ordered as their bit patterns
+        }
+    }
+}
+
+template <typename T, bool NORMS>
+static int launch_rows16(const HeadsParams& p, const HeadsGrads& g, int d, float shift, cudaStream_t s) {
+    const int rows = d == 128 ? 64 : 128;
+    const int64_t q_blocks = (int64_t)p.batch * p.heads * (g.pad_q / rows);
+    const int64_t blocks = q_blocks + (NORMS ? (int64_t)p.batch * p.kv_heads * ((p.seq_k + 127) / 128 * (128 / rows)) : 0);
+    if (blocks >= (1ll << 31)) return fail(EMMYB200_ERR_SHAPE, "attention_heads_bwd: the rows exceed the grid limit");
+    if (d == 128) heads_rows16_kernel<T, 128, NORMS><<<(unsigned)blocks, 256, 0, s>>>(p, g, shift, (int)q_blocks);
+    else heads_rows16_kernel<T, 64, NORMS><<<(unsigned)blocks, 256, 0, s>>>(p, g, shift, (int)q_blocks);
+    return launch_status("heads_rows16_kernel");
 }
 
 // ---- after it -----------------------------------------------------------------------------------------------------------
@@ -279,15 +334,17 @@ extern "C" int emmyb200_attention_heads_bwd(const emmyb200_attention_heads_desc*
     const bool tensor_cores = has_q && has_k && heads_bwd_sm100_takes(p, c->dtype, (int)c->d, g);
     const bool norms = tensor_cores && c->dtype == EMMYB200_F16;
     g.q_tiles = (int)(tensor_cores ? w.parts : (c->seq_q + kCoresTile - 1) / kCoresTile);
-    if (has_q) {
-        const int64_t blocks = (c->batch * c->heads * w.pad_q + (norms ? c->batch * c->kv_heads * c->seq_k : 0) + 7) / 8;
-        if (blocks >= (1ll << 31)) return fail(EMMYB200_ERR_SHAPE, "attention_heads_bwd: %lld rows exceed the grid limit", (long long)blocks * 8);
-        const float shift = tensor_cores ? heads_bwd_shift(c->dtype) : 0.0f;
+    if (tensor_cores) {
         if (norms) EMMY_CUDA(cudaMemsetAsync(g.amax, 0, 2 * c->batch * c->kv_heads * 4, s));
-        if (norms) heads_rows_kernel<__half, true><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d, shift);
-        else if (c->dtype == EMMYB200_F32) heads_rows_kernel<float, false><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d, shift);
-        else if (c->dtype == EMMYB200_F16) heads_rows_kernel<__half, false><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d, shift);
-        else heads_rows_kernel<__nv_bfloat16, false><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d, shift);
+        rc = norms ? launch_rows16<__half, true>(p, g, (int)c->d, heads_bwd_shift(c->dtype), s)
+                   : launch_rows16<__nv_bfloat16, false>(p, g, (int)c->d, heads_bwd_shift(c->dtype), s);
+        if (rc != EMMYB200_OK) return rc;
+    } else if (has_q) {
+        const int64_t blocks = (c->batch * c->heads * w.pad_q + 7) / 8;
+        if (blocks >= (1ll << 31)) return fail(EMMYB200_ERR_SHAPE, "attention_heads_bwd: %lld rows exceed the grid limit", (long long)blocks * 8);
+        if (c->dtype == EMMYB200_F32) heads_rows_kernel<float><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d);
+        else if (c->dtype == EMMYB200_F16) heads_rows_kernel<__half><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d);
+        else heads_rows_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, s>>>(p, g, (int)c->d);
         rc = launch_status("heads_rows_kernel");
         if (rc != EMMYB200_OK) return rc;
     }

@@ -1,21 +1,25 @@
 // Attention over heads, backward, on the tensor cores: f16 / bf16, d = 64 or 128.
 //
-// With P_ij = exp(s_ij - lse_i) and dS_ij = P_ij (dO_i . v_j - D_i), D_i = dO_i . O_i, the gradients are five products per
-// 128 x 128 tile. Two kernels recompute P, each writing what its CTAs own, so nothing is accumulated across CTAs and results
+// With P_ij = exp(s_ij - lse_i) and dS_ij = P_ij (dO_i . v_j - D_i), D_i = dO_i . O_i, the gradients are five products per tile of
+// queries x keys. Two kernels recompute P, each writing what its CTAs own, so nothing is accumulated across CTAs and results
 // are the same every time; the two score-sized products are done in both, seven in all where one kernel with atomic
 // additions into dQ would do five:
 //
-//   heads_dkv_kernel   a CTA owns 128 keys of a key head and walks the query tiles of every query head that reads it.
-//                      Everything is transposed, keys are rows: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q, with P^T
-//                      and dS^T as tensor-memory operands. 4 x 128 columns: S^T (P^T over it), dP^T (dS^T over it), dV, dK.
-//   heads_dq_kernel    a CTA owns 128 queries and walks the keys: S = Q K^T (two buffers, dS over them), dP = dO V^T,
-//                      dQ += dS K.
+//   heads_dkv_kernel   a CTA owns 128 keys of a key head and walks the queries of every query head that reads it, 64 at a
+//                      time. Everything is transposed, keys are rows: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q.
+//   heads_dq_kernel    a CTA owns 128 queries and walks the keys, 64 at a time: S = Q K^T, dP = dO V^T, dQ += dS K.
 //
-// One CTA per SM, 320 threads: warp 0 TMA (two-stage rings), warp 1 issues the products, warps 2-9 do the arithmetic between
-// them: two threads per row, 64 columns apiece, no exchange at all, since the row terms are known beforehand. A product's
-// operand (P, dS) goes back to tensor memory in two blocks of 64 columns, each over the columns its own thread has read.
-// The order of the products keeps the tensor pipe busy while the exponentials are taken: dV(i) S(i+1) dK(i) dP(i+1), and
-// dP(i+1) dQ(i) S(i+2).
+// One CTA per SM, 320 threads: warp 0 TMA (rings of 64-row stages), warp 1 issues the products, and two groups of four warps
+// do the arithmetic between them, taking the 64-column tiles in turn, one thread per row: while one group takes exponentials the products of
+// the other's tile run. Tensor memory (512 columns) sets the shape: with 128-column tiles there is room for one tile of S and dP
+// beside the accumulators, and a chain S -> exponentials -> P -> dV -> next S that left the tensor pipe idle for 40-58 % of the
+// time (measured: 3600 and 3790 cycles per 128 x 128 tile where the products take 2048 and 1536). With 64 columns S has two
+// buffers. In dkv a P tile (16 bits, 32 columns) goes back over the S tile it came from, dS beside it; in dq dS goes over dP,
+// so that the next S of a group is taken as soon as the last one is in registers.
+// A product with N = 64 would be bound by shared memory if both operands came from there (A is read again for every 64
+// columns: 48 cycles per 16-deep step against 32 of arithmetic), so the operand that stays, K in dkv, Q and dO in dq, is
+// written to tensor memory once and read from there; dkv has no room left for V.
+//   columns, dkv: S 2 x 64, dP 64, K 64, dV 128, dK 128      dq: S 2 x 64, dP 2 x 64, Q 64, dO 64, dQ 128
 //
 // Row terms come from the rows kernel already negated and shifted: nlse2 = -lse log2(e) + shift, -inf for rows that see
 // nothing or lie behind seq_q, so that P = 2^(scale log2(e) q.k + bias + nlse2) needs no test. The shift scales P by what the
@@ -43,12 +47,17 @@ struct BwdParams {
 
 __device__ uint32_t g_bwd_status;
 
+constexpr int kHalf = 64;               // columns of a tile: rows of a stage
+
 template <int D>
 struct BwdSmem {
-    static constexpr int kOperand = kTile * D * 2;
-    static constexpr int kRowsOffset = 6 * kOperand;                    // [2 stages][nlse2 128, ndelta 128]
-    static constexpr int kBarOffset = kRowsOffset + 2048;
-    static constexpr int kBiasOffset = kBarOffset + 256;
+    static constexpr int kStage = kHalf * D * 2;
+    static constexpr int kStages = 5;                                   // dkv: of Q and of dO, beside the 128 rows of V
+    static constexpr int kStagesDq = 6;                                 // dq: of K and of V
+    static constexpr int kRing = 12 * kStage;                           // either way: 2 + 2 x 5, 2 x 6 stages
+    static constexpr int kRowsOffset = kRing;                           // dkv: [stage][nlse2 64, ndelta 64]
+    static constexpr int kBarOffset = kRowsOffset + kStages * 512;
+    static constexpr int kBiasOffset = kBarOffset + 512;
     static constexpr int kSumsOffset = kBiasOffset + (int)sizeof(BiasShared);
     static constexpr int kTotal = kSumsOffset + 8 * kHeadsMaxRuns * 4 + 1024;
 };
@@ -62,50 +71,105 @@ __device__ __forceinline__ float ds_scale(const HeadsGrads& g, int64_t bk, int64
     return __int_as_float(((int)fminf(fmaxf(floorf(-log2f(bound)), -100.0f), 100.0f) + 127) << 23);
 }
 
-// Tensor-memory column of k-step kk (16 columns of a 128-column operand) inside its region: the two halves are 64 apart.
-__device__ __forceinline__ uint32_t operand_col(int kk) { return kk < 4 ? kk * 8 : 64 + (kk - 4) * 8; }
+// A row of a strided operand into tensor memory, as the A operand of a product: element pairs in columns. Rows that do not
+// exist are zeros. `cols` tensor-memory columns (two elements each) from `src`.
+template <int COLS>
+__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const uint16_t* src, bool exists) {
+    uint4 v[COLS / 4];
+#pragma unroll
+    for (int i = 0; i < COLS / 4; ++i) v[i] = exists ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < COLS / 16; ++i) {
+        uint32_t r[16];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            r[4 * k] = v[4 * i + k].x;
+            r[4 * k + 1] = v[4 * i + k].y;
+            r[4 * k + 2] = v[4 * i + k].z;
+            r[4 * k + 3] = v[4 * i + k].w;
+        }
+        ptx::tmem_st_32x32b_x16(taddr + 16 * i, r);
+    }
+}
+
+// The products of a 64-column tile, issued by a whole warp for its elected lane. B operands are stages of 64 rows: D / 64 pieces of 64 x 128 bytes.
+template <int D, bool BF16>
+struct Products {
+    static constexpr uint32_t kHi = ptx::smem_desc_sw128_hi(1024);
+    static constexpr uint32_t kPiece = kHalf * 128;
+    static constexpr uint32_t kScores = ptx::mma_idesc_f16(BF16, false, false, kTile, kHalf);
+    static constexpr uint32_t kGrads = ptx::mma_idesc_f16(BF16, false, true, kTile, D);
+    // scores: rows of A (tensor memory) times the stage's rows, contraction over the head dim
+    static __device__ __forceinline__ void scores_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t stage) {
+        const uint32_t lo = ptx::smem_desc_sw128_lo(stage, 16);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) ptx::mma_ts_lead(lead, d, a + kk * 8, lo + (((kk / 4) * kPiece + (kk % 4) * 32) >> 4), kHi, kScores, kk != 0);
+    }
+    // the same with A as 128 rows in shared memory
+    static __device__ __forceinline__ void scores_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t stage) {
+        const uint32_t lo_a = ptx::smem_desc_sw128_lo(a, 16), lo_b = ptx::smem_desc_sw128_lo(stage, 16);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+            ptx::mma_ss_lead(lead, d, lo_a + (((kk / 4) * (kTile * 128) + (kk % 4) * 32) >> 4), lo_b + (((kk / 4) * kPiece + (kk % 4) * 32) >> 4), kHi, kScores, kk != 0);
+    }
+    // gradients: A (tensor memory, 64 columns of values) times the stage, contraction over its rows
+    static __device__ __forceinline__ void grads(uint32_t lead, uint32_t d, uint32_t a, uint32_t stage, bool first) {
+        const uint32_t lo = ptx::smem_desc_sw128_lo(stage, kPiece);
+#pragma unroll
+        for (int kk = 0; kk < kHalf / 16; ++kk) ptx::mma_ts_lead(lead, d, a + kk * 8, lo + ((kk * 16 * 128) >> 4), kHi, kGrads, !first || kk != 0);
+    }
+};
+// A wait of the whole issuing warp: every lane polls, the answer is the warp's.
+__device__ __forceinline__ bool warp_spin(const WaitCtx& ctx, uint32_t bar, uint32_t parity, uint32_t code) {
+    return __all_sync(0xffffffffu, bounded_spin(ctx, bar, parity, code));
+}
 
 template <int D, bool BF16, bool BIAS>
 __global__ void __launch_bounds__(kBwdThreads, 1)
-heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                 const __grid_constant__ CUtensorMap map_do, const __grid_constant__ BwdParams p) {
+heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
+                 const __grid_constant__ BwdParams p) {
     using S = BwdSmem<D>;
-    constexpr int kChunks = D / 64;
-    constexpr uint32_t kColS = 0, kColDP = 128, kColDV = 256, kColDK = 384;
+    using Mma = Products<D, BF16>;
+    constexpr int kChunks = D / 64, kStages = S::kStages;
+    constexpr uint32_t kColS = 0, kColDP = 128, kColK = 192, kColDV = 256, kColDK = 384;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
-    const uint32_t k_smem = smem_base, v_smem = smem_base + S::kOperand;
-    auto q_smem = [&](int s) { return smem_base + (2 + s) * S::kOperand; };
-    auto do_smem = [&](int s) { return smem_base + (4 + s) * S::kOperand; };
+    const uint32_t v_smem = smem_base;
+    auto q_smem = [&](int s) { return smem_base + (2 + s) * S::kStage; };
+    auto do_smem = [&](int s) { return smem_base + (2 + kStages + s) * S::kStage; };
     const uint32_t rows_smem = smem_base + S::kRowsOffset;
     const uint32_t bar_base = smem_base + S::kBarOffset;
-    const uint32_t kv_full = bar_base, s_full = bar_base + 8, dp_full = bar_base + 16, p_ready = bar_base + 24, ds_ready = bar_base + 32,
-                   acc_full = bar_base + 40, q_full = bar_base + 48, q_empty = bar_base + 64, do_full = bar_base + 80, do_empty = bar_base + 96;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 128);
+    const uint32_t k_ready = bar_base, v_full = bar_base + 8, acc_full = bar_base + 16, s_full = bar_base + 24 /* per group */, dp_full = bar_base + 40,
+                   p_ready = bar_base + 56, ds_ready = bar_base + 72, q_full = bar_base + 128, q_empty = q_full + 8 * kStages,
+                   do_full = q_empty + 8 * kStages, do_empty = do_full + 8 * kStages;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 96);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int kt = blockIdx.x % p.k_tiles, bk = blockIdx.x / p.k_tiles;         // causal: the first key tiles see the most queries
     const int b = bk / p.h.kv_heads, hk = bk % p.h.kv_heads;
     const int key0 = kt * kTile;
     const int n_keys = heads_key_count(p.h, b), offset = heads_offset(p.h, n_keys);
-    const int first_qt = p.h.causal ? max(0, key0 - offset) / kTile : 0;       // queries before it see none of these keys
-    const int per_head = key0 < n_keys ? max(0, p.q_tiles - first_qt) : 0;
+    const int q_tiles = (p.h.seq_q + kHalf - 1) / kHalf;
+    const int first_qt = p.h.causal ? max(0, key0 - offset) / kHalf : 0;       // queries before it see none of these keys
+    const int per_head = key0 < n_keys ? max(0, q_tiles - first_qt) : 0;
     const int n_it = per_head * p.h.group;
     const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
 
     if (threadIdx.x == 0) {
-        ptx::mbar_init(kv_full, 1); ptx::mbar_init(s_full, 1); ptx::mbar_init(dp_full, 1);
-        ptx::mbar_init(p_ready, 8); ptx::mbar_init(ds_ready, 8); ptx::mbar_init(acc_full, 1);
-        for (int s = 0; s < 2; ++s) {
+        ptx::mbar_init(k_ready, 8); ptx::mbar_init(v_full, 1); ptx::mbar_init(acc_full, 1);
+        for (int x = 0; x < 2; ++x) {
+            ptx::mbar_init(s_full + 8 * x, 1); ptx::mbar_init(dp_full + 8 * x, 1); ptx::mbar_init(p_ready + 8 * x, 4); ptx::mbar_init(ds_ready + 8 * x, 4);
+        }
+        for (int s = 0; s < kStages; ++s) {
             ptx::mbar_init(q_full + 8 * s, 1); ptx::mbar_init(q_empty + 8 * s, 1);
             ptx::mbar_init(do_full + 8 * s, 1); ptx::mbar_init(do_empty + 8 * s, 1);
         }
         *abort_flag = 0;
         ptx::mbar_fence_init();
-        ptx::prefetch_tensormap(&map_q); ptx::prefetch_tensormap(&map_k); ptx::prefetch_tensormap(&map_v); ptx::prefetch_tensormap(&map_do);
+        ptx::prefetch_tensormap(&map_q); ptx::prefetch_tensormap(&map_v); ptx::prefetch_tensormap(&map_do);
     }
     if (warp == 1) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
@@ -119,165 +183,164 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (warp == 0) {
         // ---- TMA producer ------------------------------------------------------------------------------
         if (lane == 0 && n_it > 0) {
-            ptx::mbar_arrive_expect_tx(kv_full, 2 * S::kOperand);
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                ptx::tma_load_4d(k_smem + c * (kTile * 128), &map_k, kv_full, c * 64, key0, hk * p.k_at.head, b * p.k_at.batch);
-                ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, kv_full, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
-            }
+            int s = 0, gi = 0, qt = first_qt;
+            uint32_t empty = 1;
             for (int it = 0; it < n_it; ++it) {
-                const int s = it & 1, h = hk * p.h.group + it / per_head, row0 = (first_qt + it % per_head) * kTile;
-                const uint32_t empty = ((it >> 1) & 1) ^ 1;
+                const int h = hk * p.h.group + gi, row0 = qt * kHalf;
                 if (!bounded_wait(wctx, q_empty + 8 * s, empty, 0x05010000u | (it & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(q_full + 8 * s, S::kOperand + 1024);
+                ptx::mbar_arrive_expect_tx(q_full + 8 * s, S::kStage + 512);
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c)
-                    ptx::tma_load_4d(q_smem(s) + c * (kTile * 128), &map_q, q_full + 8 * s, c * 64, row0, h * p.q_at.head, b * p.q_at.batch);
+                    ptx::tma_load_4d(q_smem(s) + c * Mma::kPiece, &map_q, q_full + 8 * s, c * 64, row0, h * p.q_at.head, b * p.q_at.batch);
                 const int64_t at = ((int64_t)b * p.h.heads + h) * p.g.pad_q + row0;
-                ptx::bulk_load(rows_smem + s * 1024, p.g.lse2 + at, 512, q_full + 8 * s);
-                ptx::bulk_load(rows_smem + s * 1024 + 512, p.g.delta + at, 512, q_full + 8 * s);
+                ptx::bulk_load(rows_smem + s * 512, p.g.lse2 + at, 256, q_full + 8 * s);
+                ptx::bulk_load(rows_smem + s * 512 + 256, p.g.delta + at, 256, q_full + 8 * s);
+                if (it == 0) {
+                    ptx::mbar_arrive_expect_tx(v_full, 2 * S::kStage);
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c)
+                        ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, v_full, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
+                }
                 if (!bounded_wait(wctx, do_empty + 8 * s, empty, 0x05020000u | (it & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(do_full + 8 * s, S::kOperand);
+                ptx::mbar_arrive_expect_tx(do_full + 8 * s, S::kStage);
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c)
-                    ptx::tma_load_4d(do_smem(s) + c * (kTile * 128), &map_do, do_full + 8 * s, c * 64, row0, h * p.do_at.head, b * p.do_at.batch);
+                    ptx::tma_load_4d(do_smem(s) + c * Mma::kPiece, &map_do, do_full + 8 * s, c * 64, row0, h * p.do_at.head, b * p.do_at.batch);
+                if (++s == kStages) { s = 0; empty ^= 1; }
+                if (++qt == q_tiles) { qt = first_qt; ++gi; }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        // ---- MMA issuer ----------------------------------------------------------------------------------
-        if (lane == 0 && n_it > 0) {
-            constexpr uint32_t idesc_s = ptx::mma_idesc_f16(BF16, false, false, kTile, kTile);
-            constexpr uint32_t idesc_d = ptx::mma_idesc_f16(BF16, false, true, kTile, D);
-            // rows of `a` times rows of `b`, contraction over the head dim
-            auto scores = [&](uint32_t col, uint32_t a, uint32_t bb) {
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = (kk / 4) * (kTile * 128) + (kk % 4) * 32;
-                    ptx::mma_ss(tmem_base + col, ptx::smem_desc_sw128(a + off, 16, 1024), ptx::smem_desc_sw128(bb + off, 16, 1024), idesc_s, kk != 0);
-                }
-            };
-            // accumulator += operand in tensor memory times the rows of `bb`, contraction over those rows
-            auto grads = [&](uint32_t col, uint32_t a_col, uint32_t bb, bool first) {
-#pragma unroll
-                for (int kk = 0; kk < kTile / 16; ++kk)
-                    ptx::mma_ts(tmem_base + col, tmem_base + a_col + operand_col(kk), ptx::smem_desc_sw128(bb + kk * (16 * 128), kTile * 128, 1024), idesc_d,
-                                !first || kk != 0);
-            };
-            bool ok = bounded_spin(wctx, kv_full, 0, 0x05030000u) && bounded_spin(wctx, q_full, 0, 0x05040000u);
-            if (ok) {
+        // ---- MMA issuer: S(0) dP(0) S(1) | dV(i) dP(i+1) dK(i) S(i+2) | ... --------------------------------------
+        if (n_it > 0) {
+            const uint32_t lead = ptx::elect_lead();
+            int qs = 0, ds = 0;                                 // stages of the next S and of the next dP
+            uint32_t q_phase = 0, do_phase = 0;
+            auto s_product = [&](int it) {
+                if (!warp_spin(wctx, q_full + 8 * qs, q_phase, 0x05030000u | (it & 0xffff))) return false;
                 ptx::tc_fence_after_sync();
-                scores(kColS, k_smem, q_smem(0));
-                ptx::mma_commit(s_full);
-                ok = bounded_spin(wctx, do_full, 0, 0x05050000u);
-            }
-            if (ok) {
+                Mma::scores_ts(lead, tmem_base + kColS + 64 * (it & 1), tmem_base + kColK, q_smem(qs));
+                ptx::mma_commit_lead(lead, s_full + 8 * (it & 1));
+                if (++qs == kStages) { qs = 0; q_phase ^= 1; }
+                return true;
+            };
+            auto dp_product = [&](int it) {
+                if (!warp_spin(wctx, do_full + 8 * ds, do_phase, 0x05040000u | (it & 0xffff))) return false;
                 ptx::tc_fence_after_sync();
-                scores(kColDP, v_smem, do_smem(0));
-                ptx::mma_commit(dp_full);
-            }
+                Mma::scores_ss(lead, tmem_base + kColDP, v_smem, do_smem(ds));
+                ptx::mma_commit_lead(lead, dp_full + 8 * (it & 1));
+                if (++ds == kStages) { ds = 0; do_phase ^= 1; }
+                return true;
+            };
+            bool ok = warp_spin(wctx, k_ready, 0, 0x05050000u) && s_product(0) && warp_spin(wctx, v_full, 0, 0x05060000u) && dp_product(0);
+            if (ok && n_it > 1) ok = s_product(1);
+            int s = 0;
             for (int it = 0; it < n_it && ok; ++it) {
-                const int s = it & 1;
-                const uint32_t next = ((it + 1) >> 1) & 1;
-                if (!(ok = bounded_spin(wctx, p_ready, it & 1, 0x05060000u | (it & 0xffff)))) break;
+                const uint32_t at = tmem_base + kColS + 64 * (it & 1), phase = (it >> 1) & 1;
+                if (!(ok = warp_spin(wctx, p_ready + 8 * (it & 1), phase, 0x05070000u | (it & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
-                grads(kColDV, kColS, do_smem(s), it == 0);
-                ptx::mma_commit(do_empty + 8 * s);
-                if (it + 1 < n_it) {
-                    if (!(ok = bounded_spin(wctx, q_full + 8 * (s ^ 1), next, 0x05070000u | (it & 0xffff)))) break;
-                    ptx::tc_fence_after_sync();
-                    scores(kColS, k_smem, q_smem(s ^ 1));
-                    ptx::mma_commit(s_full);
-                }
-                if (!(ok = bounded_spin(wctx, ds_ready, it & 1, 0x05080000u | (it & 0xffff)))) break;
+                Mma::grads(lead, tmem_base + kColDV, at, do_smem(s), it == 0);
+                ptx::mma_commit_lead(lead, do_empty + 8 * s);
+                if (!(ok = warp_spin(wctx, ds_ready + 8 * (it & 1), phase, 0x05080000u | (it & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
-                grads(kColDK, kColDP, q_smem(s), it == 0);
-                ptx::mma_commit(q_empty + 8 * s);
-                if (it + 1 < n_it) {
-                    if (!(ok = bounded_spin(wctx, do_full + 8 * (s ^ 1), next, 0x05090000u | (it & 0xffff)))) break;
-                    ptx::tc_fence_after_sync();
-                    scores(kColDP, v_smem, do_smem(s ^ 1));
-                    ptx::mma_commit(dp_full);
-                }
+                if (it + 1 < n_it && !(ok = dp_product(it + 1))) break;
+                Mma::grads(lead, tmem_base + kColDK, at + 32, q_smem(s), it == 0);
+                ptx::mma_commit_lead(lead, q_empty + 8 * s);
+                if (it + 2 < n_it && !(ok = s_product(it + 2))) break;
+                if (++s == kStages) s = 0;
             }
-            if (ok) ptx::mma_commit(acc_full);
+            if (ok) ptx::mma_commit_lead(lead, acc_full);
         }
         __syncwarp();
     } else {
-        // ---- probabilities and their gradients: rows are keys, columns queries ---------------------------------------
-        const int w = warp - 2, quarter = warp & 3, half = w >> 2;
+        // ---- probabilities and their gradients: rows are keys, columns queries; group x takes tiles x, x + 2, ... ---------
+        const int w = warp - 2, quarter = warp & 3, x = w >> 2;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        const uint32_t s_at = tmem_base + lane_base + kColS + half * 64, dp_at = tmem_base + lane_base + kColDP + half * 64;
+        const uint32_t s_at = tmem_base + lane_base + kColS + x * 64, dp_at = tmem_base + lane_base + kColDP;
         const int key = key0 + quarter * 32 + lane;
+        if (n_it > 0) {                                         // K into tensor memory, half of the head dim per group
+            row_to_tmem<D / 4>(tmem_base + lane_base + kColK + x * (D / 4),
+                               static_cast<const uint16_t*>(p.g.k) + b * p.h.k_s[0] + hk * p.h.k_s[1] + key * p.h.k_s[2] + x * (D / 2), key < n_keys);
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(k_ready);
+        }
         const float g_scale = ds_scale<BF16>(p.g, bk, (int64_t)p.h.batch * p.h.kv_heads);
         const float2 g2 = make_float2(g_scale, g_scale);
         bool ok = true;
         WarpBias wb;
+        float* value = reinterpret_cast<float*>(smem_gen + S::kSumsOffset) + w * kHeadsMaxRuns;
+        if constexpr (BIAS) {
+            for (int r = lane; r < p.h.n_runs; r += 32) bias.first[r] = p.h.run_first[r];       // every warp writes the same
+        }
         int bias_head = -1;
-        for (int it = 0; it < n_it && ok; ++it) {
-            const int s = it & 1;
-            const int q0 = (first_qt + it % per_head) * kTile + half * 64;      // this thread's first query
-            float c = p.h.scale_log2, add = 0.0f;
+        int gi = 0, qt = first_qt, s = x;                       // this group's tile and its stage
+        uint32_t q_phase = 0;
+        if (x == 1 && ++qt == q_tiles) { qt = first_qt; ++gi; }
+        for (int it = x; it < n_it && ok; it += 2) {
+            const uint32_t phase = (it >> 1) & 1;
+            const int q0 = qt * kHalf;                          // this thread's first query
+            const float c = p.h.scale_log2;
             bool looked_up = false;
             if constexpr (BIAS) {
                 // the table's column changes with the query head; every warp keeps a copy of its own, so that no two warps have to meet
-                const int h = hk * p.h.group + it / per_head;
+                const int h = hk * p.h.group + gi;
                 if (h != bias_head) {
                     bias_head = h;
                     __syncwarp();
-                    float* value = reinterpret_cast<float*>(smem_gen + S::kSumsOffset) + w * kHeadsMaxRuns;
-                    for (int r = lane; r < p.h.n_runs; r += 32) {
-                        if (it == 0) bias.first[r] = p.h.run_first[r];          // every warp writes the same
-                        value[r] = heads_run_bias(p.h, r, h);
-                    }
+                    for (int r = lane; r < p.h.n_runs; r += 32) value[r] = heads_run_bias(p.h, r, h);
                     __syncwarp();
                     wb.reset();
                 }
-                looked_up = !wb.block(bias, reinterpret_cast<float*>(smem_gen + S::kSumsOffset) + w * kHeadsMaxRuns, w, lane, p.h.n_runs,
-                                      key0 + quarter * 32 - (q0 + 63 + offset));
-                add = wb.same;
+                looked_up = !wb.block(bias, value, w, lane, p.h.n_runs, key0 + quarter * 32 - (q0 + 63 + offset));
             }
-            ok = __all_sync(0xffffffffu, bounded_wait(wctx, q_full + 8 * s, (it >> 1) & 1, 0x050a0000u | (it & 0xffff)) &&
-                                             bounded_wait(wctx, s_full, it & 1, 0x050b0000u | (it & 0xffff)));
+            ok = __all_sync(0xffffffffu, bounded_wait(wctx, q_full + 8 * s, q_phase, 0x050a0000u | (it & 0xffff)) &&
+                                             bounded_wait(wctx, s_full + 8 * x, phase, 0x050b0000u | (it & 0xffff)));
             if (!ok) break;
             ptx::tc_fence_after_sync();
-            const float4* nlse = reinterpret_cast<const float4*>(smem_gen + S::kRowsOffset + s * 1024 + half * 256);
-            const float4* ndelta = nlse + 32;
+            const float4* nlse = reinterpret_cast<const float4*>(smem_gen + S::kRowsOffset + s * 512);
+            const float4* ndelta = nlse + 16;
             // columns below `hidden` are not seen: queries before the key, or the whole row for keys behind the count
             const int hidden = key >= n_keys ? 64 : (p.h.causal ? key - offset - q0 : 0);
             const bool masked = __any_sync(0xffffffffu, hidden > 0);
             float2 e[32];
+            uint32_t r[64];
+            ptx::tmem_ld_32x32b_x32(s_at, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+            ptx::tmem_ld_32x32b_x32(s_at + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+            ptx::tmem_ld_wait();
+            float cc = c, aa = 0.0f;
+            if constexpr (BIAS) {
+                aa = wb.same;
+                if (looked_up) {
+                    const float* at = bias.by_dist[w] + 63 + lane;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) r[i] = __float_as_uint(fmaf(__uint_as_float(r[i]), c, at[-i]));
+                    cc = 1.0f;
+                    aa = 0.0f;
+                }
+            }
+            const float2 c2 = make_float2(cc, cc), a2 = make_float2(aa, aa);
 #pragma unroll
             for (int ch = 0; ch < 2; ++ch) {
-                uint32_t r[32];
-                ptx::tmem_ld_32x32b_x32(s_at + ch * 32, r);
-                ptx::tmem_ld_wait();
-                if constexpr (BIAS) {
-                    if (looked_up) {
-                        const float* at = bias.by_dist[w] + 63 + lane - ch * 32;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(fmaf(__uint_as_float(r[i]), c, at[-i]));
-                    }
-                }
-                const float cc = BIAS && looked_up ? 1.0f : c, aa = BIAS && looked_up ? 0.0f : add;
-                const float2 c2 = make_float2(cc, cc), a2 = make_float2(aa, aa);
-                uint32_t pk[16];
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    float4 nl = nlse[ch * 8 + i / 2];
+                for (int i = ch * 16; i < ch * 16 + 16; i += 2) {
+                    const float4 nl = nlse[i / 2];
                     float2 n0 = make_float2(nl.x, nl.y), n1 = make_float2(nl.z, nl.w);
                     if constexpr (BIAS) { n0 = add2(n0, a2); n1 = add2(n1, a2); }
                     const float2 y0 = fma2(f2(r[2 * i], r[2 * i + 1]), c2, n0), y1 = fma2(f2(r[2 * i + 2], r[2 * i + 3]), c2, n1);
-                    e[ch * 16 + i] = make_float2(ptx::ex2_approx(y0.x), ptx::ex2_approx(y0.y));
-                    e[ch * 16 + i + 1] = make_float2(ptx::ex2_approx(y1.x), ptx::ex2_approx(y1.y));
+                    e[i] = make_float2(ptx::ex2_approx(y0.x), ptx::ex2_approx(y0.y));
+                    e[i + 1] = make_float2(ptx::ex2_approx(y1.x), ptx::ex2_approx(y1.y));
                 }
                 if (masked) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (ch * 32 + 2 * i < hidden) e[ch * 16 + i].x = 0.0f;
-                        if (ch * 32 + 2 * i + 1 < hidden) e[ch * 16 + i].y = 0.0f;
+                    for (int i = ch * 16; i < ch * 16 + 16; ++i) {
+                        if (2 * i < hidden) e[i].x = 0.0f;
+                        if (2 * i + 1 < hidden) e[i].y = 0.0f;
                     }
                 }
+                uint32_t pk[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) pk[i] = operand_pair<BF16>(e[ch * 16 + i]);
                 ptx::tmem_st_32x32b_x16(s_at + ch * 16, pk);
@@ -285,59 +348,63 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(p_ready);
-            ok = __all_sync(0xffffffffu, bounded_wait(wctx, dp_full, it & 1, 0x050c0000u | (it & 0xffff)));
+            if (lane == 0) ptx::mbar_arrive(p_ready + 8 * x);
+            ok = __all_sync(0xffffffffu, bounded_wait(wctx, dp_full + 8 * x, phase, 0x050c0000u | (it & 0xffff)));
             if (!ok) break;
             ptx::tc_fence_after_sync();
+            ptx::tmem_ld_32x32b_x32(dp_at, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+            ptx::tmem_ld_32x32b_x32(dp_at + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+            ptx::tmem_ld_wait();
 #pragma unroll
             for (int ch = 0; ch < 2; ++ch) {
-                uint32_t r[32], pk[16];
-                ptx::tmem_ld_32x32b_x32(dp_at + ch * 32, r);
-                ptx::tmem_ld_wait();
+                uint32_t pk[16];
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float4 nd = ndelta[ch * 8 + i / 2];
-                    float2 e0 = e[ch * 16 + i], e1 = e[ch * 16 + i + 1];
+                for (int i = ch * 16; i < ch * 16 + 16; i += 2) {
+                    const float4 nd = ndelta[i / 2];
+                    float2 e0 = e[i], e1 = e[i + 1];
                     if constexpr (!BF16) { e0 = mul2(e0, g2); e1 = mul2(e1, g2); }
                     float2 d0 = mul2(e0, add2(f2(r[2 * i], r[2 * i + 1]), make_float2(nd.x, nd.y)));
                     float2 d1 = mul2(e1, add2(f2(r[2 * i + 2], r[2 * i + 3]), make_float2(nd.z, nd.w)));
                     if (masked) {                                       // dP may hold anything there
-                        if (ch * 32 + 2 * i < hidden) d0.x = 0.0f;
-                        if (ch * 32 + 2 * i + 1 < hidden) d0.y = 0.0f;
-                        if (ch * 32 + 2 * i + 2 < hidden) d1.x = 0.0f;
-                        if (ch * 32 + 2 * i + 3 < hidden) d1.y = 0.0f;
+                        if (2 * i < hidden) d0.x = 0.0f;
+                        if (2 * i + 1 < hidden) d0.y = 0.0f;
+                        if (2 * i + 2 < hidden) d1.x = 0.0f;
+                        if (2 * i + 3 < hidden) d1.y = 0.0f;
                     }
-                    pk[i] = operand_pair<BF16>(d0);
-                    pk[i + 1] = operand_pair<BF16>(d1);
+                    pk[i - ch * 16] = operand_pair<BF16>(d0);
+                    pk[i - ch * 16 + 1] = operand_pair<BF16>(d1);
                 }
-                ptx::tmem_st_32x32b_x16(dp_at + ch * 16, pk);
+                ptx::tmem_st_32x32b_x16(s_at + 32 + ch * 16, pk);
             }
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(ds_ready);
+            if (lane == 0) ptx::mbar_arrive(ds_ready + 8 * x);
+            // two tiles on
+            s += 2;
+            if (s >= kStages) { s -= kStages; q_phase ^= 1; }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (++qt == q_tiles) { qt = first_qt; ++gi; }
         }
         if (ok && n_it > 0) ok = __all_sync(0xffffffffu, bounded_wait(wctx, acc_full, 0, 0x050d0000u));
-        if (ok) {
+        if (ok) {                                               // group 0 writes dV, group 1 dK
             ptx::tc_fence_after_sync();
-            const float dv_scale = BF16 ? 1.0f : 1.0f / (1 << kF16Shift), dk_scale = dv_scale * p.h.scale / g_scale;
-            uint16_t* dv = static_cast<uint16_t*>(p.g.dv) + b * p.h.dv_s[0] + hk * p.h.dv_s[1] + key * p.h.dv_s[2] + half * (D / 2);
-            uint16_t* dk = static_cast<uint16_t*>(p.g.dk) + b * p.h.dk_s[0] + hk * p.h.dk_s[1] + key * p.h.dk_s[2] + half * (D / 2);
+            const float f = (BF16 ? 1.0f : 1.0f / (1 << kF16Shift)) * (x ? p.h.scale / g_scale : 1.0f);
+            uint16_t* out = x ? static_cast<uint16_t*>(p.g.dk) + b * p.h.dk_s[0] + hk * p.h.dk_s[1] + key * p.h.dk_s[2]
+                              : static_cast<uint16_t*>(p.g.dv) + b * p.h.dv_s[0] + hk * p.h.dv_s[1] + key * p.h.dv_s[2];
 #pragma unroll 1
-            for (int ch = 0; ch < 2 * (D / 64); ++ch) {                 // dV's, then dK's pieces of 32 columns
-                const bool is_dk = ch >= D / 64;
-                const int col = (is_dk ? ch - D / 64 : ch) * 32;
+            for (int col = 0; col < D; col += 32) {
                 uint32_t r[32];
                 if (n_it > 0) {
-                    ptx::tmem_ld_32x32b_x32(tmem_base + lane_base + (is_dk ? kColDK : kColDV) + half * (D / 2) + col, r);
+                    ptx::tmem_ld_32x32b_x32(tmem_base + lane_base + (x ? kColDK : kColDV) + col, r);
                     ptx::tmem_ld_wait();
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) r[i] = 0;
                 }
-                const float f = is_dk ? dk_scale : dv_scale;
                 if (key < p.h.seq_k) {
-                    uint4* dst = reinterpret_cast<uint4*>((is_dk ? dk : dv) + col);
+                    uint4* dst = reinterpret_cast<uint4*>(out + col);
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         uint32_t v[4];
@@ -379,44 +446,45 @@ struct RunSums {
 
 template <int D, bool BF16, bool BIAS>
 __global__ void __launch_bounds__(kBwdThreads, 1)
-heads_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                const __grid_constant__ CUtensorMap map_do, const __grid_constant__ BwdParams p) {
+heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ BwdParams p) {
     using S = BwdSmem<D>;
-    constexpr int kChunks = D / 64;
-    constexpr uint32_t kColS = 0, kColDP = 256, kColDQ = 384;           // S: two buffers of 128 columns
+    using Mma = Products<D, BF16>;
+    constexpr int kChunks = D / 64, kStages = S::kStagesDq;
+    constexpr uint32_t kColS = 0, kColDP = 128, kColQ = 256, kColDO = 320, kColDQ = 384;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
-    const uint32_t q_smem = smem_base, do_smem = smem_base + S::kOperand;
-    auto k_smem = [&](int s) { return smem_base + (2 + s) * S::kOperand; };
-    auto v_smem = [&](int s) { return smem_base + (4 + s) * S::kOperand; };
+    auto k_smem = [&](int s) { return smem_base + s * S::kStage; };
+    auto v_smem = [&](int s) { return smem_base + (kStages + s) * S::kStage; };
     const uint32_t bar_base = smem_base + S::kBarOffset;
-    const uint32_t q_full = bar_base, do_full = bar_base + 8, s_full = bar_base + 16 /* two */, dp_full = bar_base + 32, ds_ready = bar_base + 40,
-                   acc_full = bar_base + 48, k_full = bar_base + 64, k_empty = bar_base + 80, v_full = bar_base + 96, v_empty = bar_base + 112;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 128);
+    const uint32_t a_ready = bar_base, acc_full = bar_base + 8, s_full = bar_base + 16 /* per group */, dp_full = bar_base + 32, ds_ready = bar_base + 48, s_free = bar_base + 64,
+                   k_full = bar_base + 128, k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 96);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int bh = blockIdx.x / p.q_tiles;
     const int qt = p.h.causal ? p.q_tiles - 1 - (int)(blockIdx.x % p.q_tiles) : (int)(blockIdx.x % p.q_tiles);
     const int b = bh / p.h.heads, h = bh % p.h.heads, hk = h / p.h.group;
     const int row0 = qt * kTile;
     const int n_keys = heads_key_count(p.h, b), offset = heads_offset(p.h, n_keys);
     const int key_end = p.h.causal ? max(0, min(n_keys, min(row0 + kTile, p.h.seq_q) + offset)) : n_keys;
-    const int n_it = (key_end + kTile - 1) / kTile;
+    const int n_it = (key_end + kHalf - 1) / kHalf;
     const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
 
     if (threadIdx.x == 0) {
-        ptx::mbar_init(q_full, 1); ptx::mbar_init(do_full, 1); ptx::mbar_init(s_full, 1); ptx::mbar_init(s_full + 8, 1);
-        ptx::mbar_init(dp_full, 1); ptx::mbar_init(ds_ready, 8); ptx::mbar_init(acc_full, 1);
-        for (int s = 0; s < 2; ++s) {
+        ptx::mbar_init(a_ready, 8); ptx::mbar_init(acc_full, 1);
+        for (int x = 0; x < 2; ++x) {
+            ptx::mbar_init(s_full + 8 * x, 1); ptx::mbar_init(dp_full + 8 * x, 1); ptx::mbar_init(ds_ready + 8 * x, 4); ptx::mbar_init(s_free + 8 * x, 4);
+        }
+        for (int s = 0; s < kStages; ++s) {
             ptx::mbar_init(k_full + 8 * s, 1); ptx::mbar_init(k_empty + 8 * s, 1);
             ptx::mbar_init(v_full + 8 * s, 1); ptx::mbar_init(v_empty + 8 * s, 1);
         }
         *abort_flag = 0;
         ptx::mbar_fence_init();
-        ptx::prefetch_tensormap(&map_q); ptx::prefetch_tensormap(&map_k); ptx::prefetch_tensormap(&map_v); ptx::prefetch_tensormap(&map_do);
+        ptx::prefetch_tensormap(&map_k); ptx::prefetch_tensormap(&map_v);
     }
     if (BIAS) load_bias(bias, p.h, h, threadIdx.x, kBwdThreads);
     if (warp == 1) {
@@ -430,80 +498,83 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
     if (warp == 0) {
         // ---- TMA producer ------------------------------------------------------------------------------
-        if (lane == 0 && n_it > 0) {
-            ptx::mbar_arrive_expect_tx(q_full, S::kOperand);
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c) ptx::tma_load_4d(q_smem + c * (kTile * 128), &map_q, q_full, c * 64, row0, h * p.q_at.head, b * p.q_at.batch);
+        if (lane == 0) {
+            int s = 0;
+            uint32_t empty = 1;
             for (int it = 0; it < n_it; ++it) {
-                const int s = it & 1, key0 = it * kTile;
-                const uint32_t empty = ((it >> 1) & 1) ^ 1;
+                const int key0 = it * kHalf;
                 if (!bounded_wait(wctx, k_empty + 8 * s, empty, 0x06010000u | (it & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(k_full + 8 * s, S::kOperand);
+                ptx::mbar_arrive_expect_tx(k_full + 8 * s, S::kStage);
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c)
-                    ptx::tma_load_4d(k_smem(s) + c * (kTile * 128), &map_k, k_full + 8 * s, c * 64, key0, hk * p.k_at.head, b * p.k_at.batch);
-                if (it == 0) {
-                    ptx::mbar_arrive_expect_tx(do_full, S::kOperand);
-#pragma unroll
-                    for (int c = 0; c < kChunks; ++c)
-                        ptx::tma_load_4d(do_smem + c * (kTile * 128), &map_do, do_full, c * 64, row0, h * p.do_at.head, b * p.do_at.batch);
-                }
+                    ptx::tma_load_4d(k_smem(s) + c * Mma::kPiece, &map_k, k_full + 8 * s, c * 64, key0, hk * p.k_at.head, b * p.k_at.batch);
                 if (!bounded_wait(wctx, v_empty + 8 * s, empty, 0x06020000u | (it & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(v_full + 8 * s, S::kOperand);
+                ptx::mbar_arrive_expect_tx(v_full + 8 * s, S::kStage);
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c)
-                    ptx::tma_load_4d(v_smem(s) + c * (kTile * 128), &map_v, v_full + 8 * s, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
+                    ptx::tma_load_4d(v_smem(s) + c * Mma::kPiece, &map_v, v_full + 8 * s, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
+                if (++s == kStages) { s = 0; empty ^= 1; }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        // ---- MMA issuer ----------------------------------------------------------------------------------
-        if (lane == 0 && n_it > 0) {
-            constexpr uint32_t idesc_s = ptx::mma_idesc_f16(BF16, false, false, kTile, kTile);
-            constexpr uint32_t idesc_d = ptx::mma_idesc_f16(BF16, false, true, kTile, D);
-            auto scores = [&](uint32_t col, uint32_t a, uint32_t bb) {
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = (kk / 4) * (kTile * 128) + (kk % 4) * 32;
-                    ptx::mma_ss(tmem_base + col, ptx::smem_desc_sw128(a + off, 16, 1024), ptx::smem_desc_sw128(bb + off, 16, 1024), idesc_s, kk != 0);
-                }
-            };
+        // ---- MMA issuer: S(0) dP(0) S(1) dP(1) | S(i+2) dQ(i) dP(i+2) | ... ------------------------------------------
+        if (n_it > 0) {
+            const uint32_t lead = ptx::elect_lead();
+            int ks = 0, vs = 0;                                 // stages of the next S and of the next dP
+            uint32_t k_phase = 0, v_phase = 0;
             auto s_product = [&](int it) {
-                if (!bounded_spin(wctx, k_full + 8 * (it & 1), (it >> 1) & 1, 0x06030000u | (it & 0xffff))) return false;
+                if (!warp_spin(wctx, k_full + 8 * ks, k_phase, 0x06030000u | (it & 0xffff))) return false;
                 ptx::tc_fence_after_sync();
-                scores(kColS + 128 * (it & 1), q_smem, k_smem(it & 1));
-                ptx::mma_commit(s_full + 8 * (it & 1));
+                Mma::scores_ts(lead, tmem_base + kColS + 64 * (it & 1), tmem_base + kColQ, k_smem(ks));
+                ptx::mma_commit_lead(lead, s_full + 8 * (it & 1));
+                if (++ks == kStages) { ks = 0; k_phase ^= 1; }
                 return true;
             };
             auto dp_product = [&](int it) {
-                if (!bounded_spin(wctx, v_full + 8 * (it & 1), (it >> 1) & 1, 0x06040000u | (it & 0xffff))) return false;
+                if (!warp_spin(wctx, v_full + 8 * vs, v_phase, 0x06040000u | (it & 0xffff))) return false;
                 ptx::tc_fence_after_sync();
-                scores(kColDP, do_smem, v_smem(it & 1));
-                ptx::mma_commit(v_empty + 8 * (it & 1));
-                ptx::mma_commit(dp_full);
+                Mma::scores_ts(lead, tmem_base + kColDP + 64 * (it & 1), tmem_base + kColDO, v_smem(vs));
+                ptx::mma_commit_lead(lead, dp_full + 8 * (it & 1));
+                ptx::mma_commit_lead(lead, v_empty + 8 * vs);
+                if (++vs == kStages) { vs = 0; v_phase ^= 1; }
                 return true;
             };
-            bool ok = bounded_spin(wctx, q_full, 0, 0x06050000u) && s_product(0) && bounded_spin(wctx, do_full, 0, 0x06060000u) && dp_product(0);
-            if (ok && n_it > 1) ok = s_product(1);
+            bool ok = warp_spin(wctx, a_ready, 0, 0x06050000u) && s_product(0) && dp_product(0);
+            if (ok && n_it > 1) ok = s_product(1) && dp_product(1);
+            int s = 0;
             for (int it = 0; it < n_it && ok; ++it) {
-                if (!(ok = bounded_spin(wctx, ds_ready, it & 1, 0x06070000u | (it & 0xffff)))) break;
+                const uint32_t phase = (it >> 1) & 1;
+                if (it + 2 < n_it) {                            // S(it) is in registers: its columns are free
+                    if (!(ok = warp_spin(wctx, s_free + 8 * (it & 1), phase, 0x06060000u | (it & 0xffff)))) break;
+                    if (!(ok = s_product(it + 2))) break;
+                }
+                if (!(ok = warp_spin(wctx, ds_ready + 8 * (it & 1), phase, 0x06070000u | (it & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
-                if (it + 1 < n_it && !(ok = dp_product(it + 1))) break;
-#pragma unroll
-                for (int kk = 0; kk < kTile / 16; ++kk)         // dQ += dS K, contraction over the keys
-                    ptx::mma_ts(tmem_base + kColDQ, tmem_base + kColS + 128 * (it & 1) + operand_col(kk),
-                                ptx::smem_desc_sw128(k_smem(it & 1) + kk * (16 * 128), kTile * 128, 1024), idesc_d, (it | kk) != 0);
-                ptx::mma_commit(k_empty + 8 * (it & 1));
-                if (it + 2 < n_it && !(ok = s_product(it + 2))) break;
+                Mma::grads(lead, tmem_base + kColDQ, tmem_base + kColDP + 64 * (it & 1), k_smem(s), it == 0);
+                ptx::mma_commit_lead(lead, k_empty + 8 * s);
+                if (it + 2 < n_it && !(ok = dp_product(it + 2))) break;
+                if (++s == kStages) s = 0;
             }
-            if (ok) ptx::mma_commit(acc_full);
+            if (ok) ptx::mma_commit_lead(lead, acc_full);
         }
         __syncwarp();
     } else {
-        // ---- probabilities and their gradients: rows are queries, columns keys ---------------------------------------
-        const int w = warp - 2, quarter = warp & 3, half = w >> 2;
+        // ---- probabilities and their gradients: rows are queries, columns keys; group x takes tiles x, x + 2, ... --------
+        const int w = warp - 2, quarter = warp & 3, x = w >> 2;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        const uint32_t s_at = tmem_base + lane_base + kColS + x * 64, dp_at = tmem_base + lane_base + kColDP + x * 64;
         const int row = row0 + quarter * 32 + lane;
+        if (n_it > 0) {                                         // group 0 writes Q to tensor memory, group 1 dO
+            row_to_tmem<D / 2>(tmem_base + lane_base + (x ? kColDO : kColQ),
+                               x ? static_cast<const uint16_t*>(p.g.d_o) + b * p.h.do_s[0] + h * p.h.do_s[1] + row * p.h.do_s[2]
+                                 : static_cast<const uint16_t*>(p.g.q) + b * p.h.q_s[0] + h * p.h.q_s[1] + row * p.h.q_s[2],
+                               row < p.h.seq_q);
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(a_ready);
+        }
         const int64_t at_row = (int64_t)bh * p.g.pad_q + row;
         const float nlse = p.g.lse2[at_row], ndelta = p.g.delta[at_row];
         const float g_scale = ds_scale<BF16>(p.g, b * p.h.kv_heads + hk, (int64_t)p.h.batch * p.h.kv_heads);
@@ -519,103 +590,92 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             for (int r = lane; r < p.h.n_runs; r += 32) sums[r] = 0.0f;
             __syncwarp();
         }
-        for (int it = 0; it < n_it && ok; ++it) {
-            const int key0 = it * kTile + half * 64;            // this thread's first key
-            const uint32_t s_at = tmem_base + lane_base + kColS + 128 * (it & 1) + half * 64, dp_at = tmem_base + lane_base + kColDP + half * 64;
+        int s = x;                                              // the tile's stage
+        for (int it = x; it < n_it && ok; it += 2) {
+            const uint32_t phase = (it >> 1) & 1;
+            const int key0 = it * kHalf;
             const int d0 = key0 - (row0 + quarter * 32 + 31 + offset);
             float c = p.h.scale_log2, add = nlse;
             bool looked_up = false;
             if constexpr (BIAS) looked_up = !wb.block(bias, bias.value, w, lane, p.h.n_runs, d0);
-            ok = __all_sync(0xffffffffu, bounded_wait(wctx, s_full + 8 * (it & 1), (it >> 1) & 1, 0x06080000u | (it & 0xffff)));
+            ok = __all_sync(0xffffffffu, bounded_wait(wctx, s_full + 8 * x, phase, 0x06080000u | (it & 0xffff)));
             if (!ok) break;
             ptx::tc_fence_after_sync();
-            const int valid = sees - key0;                      // of this thread's columns
+            const int valid = sees - key0;                      // columns that are seen
             const bool masked = __any_sync(0xffffffffu, valid < 64);
             float2 e[32];
+            uint32_t r[64];
+            ptx::tmem_ld_32x32b_x32(s_at, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+            ptx::tmem_ld_32x32b_x32(s_at + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+            ptx::tmem_ld_wait();
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(s_free + 8 * x);
+            if constexpr (BIAS) {
+                if (looked_up) {
+                    const float* at = bias.by_dist[w] + 31 - lane;
 #pragma unroll
-            for (int ch = 0; ch < 2; ++ch) {
-                uint32_t r[32];
-                ptx::tmem_ld_32x32b_x32(s_at + ch * 32, r);
-                ptx::tmem_ld_wait();
-                float cc = c, aa = add;
-                if constexpr (BIAS) {
-                    if (looked_up) {
-                        const float* at = bias.by_dist[w] + 31 - lane + ch * 32;
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(fmaf(__uint_as_float(r[i]), c, at[i]));
-                        cc = 1.0f;
-                    } else {
-                        aa = add + wb.same;
-                    }
+                    for (int i = 0; i < 64; ++i) r[i] = __float_as_uint(fmaf(__uint_as_float(r[i]), c, at[i]));
+                    c = 1.0f;
+                } else {
+                    add += wb.same;
                 }
-                const float2 c2 = make_float2(cc, cc), a2 = make_float2(aa, aa);
+            }
+            const float2 c2 = make_float2(c, c), a2 = make_float2(add, add);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float2 y = fma2(f2(r[2 * i], r[2 * i + 1]), c2, a2);
-                    e[ch * 16 + i] = make_float2(ptx::ex2_approx(y.x), ptx::ex2_approx(y.y));
-                }
+            for (int i = 0; i < 32; ++i) {
+                const float2 y = fma2(f2(r[2 * i], r[2 * i + 1]), c2, a2);
+                e[i] = make_float2(ptx::ex2_approx(y.x), ptx::ex2_approx(y.y));
             }
             // K rows behind the key count hold whatever the caller left there: cleared before dQ's product multiplies them by dS's zeros
-            const int live = n_keys - it * kTile;
-            if (live < kTile && n_keys < p.h.seq_k) {           // S has been computed from them; its columns there are not used
-                for (int x = live * 8 + (int)threadIdx.x - 64; x < kTile * 8; x += 256)
+            const int live = n_keys - key0;
+            if (live < kHalf && n_keys < p.h.seq_k) {           // S has been computed from them; its columns there are not used
+                for (int k = live * 8 + (quarter * 32 + lane); k < kHalf * 8; k += 128)
 #pragma unroll
                     for (int ch = 0; ch < kChunks; ++ch)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(k_smem(it & 1) + ch * (kTile * 128) + x * 16), "r"(0) : "memory");
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(k_smem(s) + ch * Mma::kPiece + k * 16), "r"(0) : "memory");
                 ptx::fence_proxy_async_smem();
             }
-            ok = __all_sync(0xffffffffu, bounded_wait(wctx, dp_full, it & 1, 0x06090000u | (it & 0xffff)));
+            ok = __all_sync(0xffffffffu, bounded_wait(wctx, dp_full + 8 * x, phase, 0x06090000u | (it & 0xffff)));
             if (!ok) break;
             ptx::tc_fence_after_sync();
-            float diag = 0.0f;                                  // a diagonal's partial sum, passing through this lane
-            float2 same_sum = make_float2(0.0f, 0.0f);
-            if (BIAS && looked_up) __syncwarp();                // the biases have been read: the diagonal sums take their place
+            ptx::tmem_ld_32x32b_x32(dp_at, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+            ptx::tmem_ld_32x32b_x32(dp_at + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+            ptx::tmem_ld_wait();
 #pragma unroll
             for (int ch = 0; ch < 2; ++ch) {
-                uint32_t r[32], pk[16];
-                ptx::tmem_ld_32x32b_x32(dp_at + ch * 32, r);
-                ptx::tmem_ld_wait();
+                uint32_t pk[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float2 ee = e[ch * 16 + i];
+                for (int i = ch * 16; i < ch * 16 + 16; ++i) {
+                    float2 ee = e[i];
                     if constexpr (!BF16) ee = mul2(ee, g2);
                     float2 ds = mul2(ee, add2(f2(r[2 * i], r[2 * i + 1]), nd2));
                     if (masked) {
-                        if (ch * 32 + 2 * i >= valid) ds.x = 0.0f;
-                        if (ch * 32 + 2 * i + 1 >= valid) ds.y = 0.0f;
+                        if (2 * i >= valid) ds.x = 0.0f;
+                        if (2 * i + 1 >= valid) ds.y = 0.0f;
                     }
-                    pk[i] = operand_pair<BF16>(ds);
+                    pk[i - ch * 16] = operand_pair<BF16>(ds);
                     if constexpr (BIAS) {
                         r[2 * i] = __float_as_uint(ds.x);
                         r[2 * i + 1] = __float_as_uint(ds.y);
                     }
                 }
-                ptx::tmem_st_32x32b_x16(s_at + ch * 16, pk);
-                if (ch == 1) {
-                    ptx::tmem_st_wait();
-                    ptx::tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(ds_ready);
-                }
-                if constexpr (BIAS) {
-                    if (want_bias) {
-                        if (looked_up) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const float below = __shfl_up_sync(0xffffffffu, diag, 1);
-                                diag = (lane == 0 ? 0.0f : below) + __uint_as_float(r[i]);
-                                if (lane == 31) bias.by_dist[w][ch * 32 + i] = diag;
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) same_sum = add2(same_sum, f2(r[2 * i], r[2 * i + 1]));
-                        }
-                    }
-                }
+                ptx::tmem_st_32x32b_x16(dp_at + ch * 16, pk);
             }
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ds_ready + 8 * x);
             if constexpr (BIAS) {
                 if (want_bias) {
-                    if (looked_up) {
+                    if (looked_up) {                            // the biases have been read: the diagonal sums take their place
+                        float diag = 0.0f;                      // a diagonal's partial sum, passing through this lane
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) {
+                            const float below = __shfl_up_sync(0xffffffffu, diag, 1);
+                            diag = (lane == 0 ? 0.0f : below) + __uint_as_float(r[i]);
+                            if (lane == 31) bias.by_dist[w][i] = diag;
+                        }
                         if (lane < 31) bias.by_dist[w][94 - lane] = diag;
                         __syncwarp();
                         // runs the block touches, one lane each
@@ -633,22 +693,28 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                             __syncwarp();
                             rs.run = wb.run;
                         }
-                        rs.acc += same_sum.x + same_sum.y;
+                        float2 part[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) part[i & 3] = add2(part[i & 3], f2(r[2 * i], r[2 * i + 1]));
+                        const float2 sum = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+                        rs.acc += sum.x + sum.y;
                     }
                 }
             }
+            s += 2;
+            if (s >= kStages) s -= kStages;
         }
         if (ok && n_it > 0) ok = __all_sync(0xffffffffu, bounded_wait(wctx, acc_full, 0, 0x060a0000u));
         if (ok) {
             ptx::tc_fence_after_sync();
             const float out = BF16 ? 1.0f : 1.0f / ((1 << kF16Shift) * g_scale);
             const float f = p.h.scale * out;
-            uint16_t* dq = static_cast<uint16_t*>(p.g.dq) + b * p.h.dq_s[0] + h * p.h.dq_s[1] + row * p.h.dq_s[2] + half * (D / 2);
+            uint16_t* dq = static_cast<uint16_t*>(p.g.dq) + b * p.h.dq_s[0] + h * p.h.dq_s[1] + row * p.h.dq_s[2] + x * (D / 2);
 #pragma unroll 1
             for (int ch = 0; ch < D / 64; ++ch) {
                 uint32_t r[32];
                 if (n_it > 0) {
-                    ptx::tmem_ld_32x32b_x32(tmem_base + lane_base + kColDQ + half * (D / 2) + ch * 32, r);
+                    ptx::tmem_ld_32x32b_x32(tmem_base + lane_base + kColDQ + x * (D / 2) + ch * 32, r);
                     ptx::tmem_ld_wait();
                 } else {
 #pragma unroll
@@ -691,11 +757,12 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 template <int D, bool BF16>
 static int launch_bwd(BwdParams& p, cudaStream_t s) {
     const HeadsParams& h = p.h;
-    CUtensorMap mq, mk, mv, mdo;
-    int rc = make_map(&mq, &p.q_at, p.g.q, h.batch, h.heads, h.seq_q, D, h.q_s, kTile, 1);
-    if (rc == EMMYB200_OK) rc = make_map(&mk, &p.k_at, p.g.k, h.batch, h.kv_heads, h.seq_k, D, h.k_s, kTile, 1);
-    if (rc == EMMYB200_OK) rc = make_map(&mv, &p.v_at, p.g.v, h.batch, h.kv_heads, h.seq_k, D, h.v_s, kTile, 1);
-    if (rc == EMMYB200_OK) rc = make_map(&mdo, &p.do_at, p.g.d_o, h.batch, h.heads, h.seq_q, D, h.do_s, kTile, 1);
+    CUtensorMap mq, mk, mv, mv_tile, mdo;
+    int rc = make_map(&mq, &p.q_at, p.g.q, h.batch, h.heads, h.seq_q, D, h.q_s, kHalf, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&mk, &p.k_at, p.g.k, h.batch, h.kv_heads, h.seq_k, D, h.k_s, kHalf, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&mv, &p.v_at, p.g.v, h.batch, h.kv_heads, h.seq_k, D, h.v_s, kHalf, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&mv_tile, &p.v_at, p.g.v, h.batch, h.kv_heads, h.seq_k, D, h.v_s, kTile, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&mdo, &p.do_at, p.g.d_o, h.batch, h.heads, h.seq_q, D, h.do_s, kHalf, 1);
     if (rc != EMMYB200_OK) return rc;
     EMMY_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p.status), g_bwd_status));
     const int64_t kv_ctas = (int64_t)h.batch * h.kv_heads * p.k_tiles, q_ctas = (int64_t)h.batch * h.heads * p.q_tiles;
@@ -704,10 +771,10 @@ static int launch_bwd(BwdParams& p, cudaStream_t s) {
     auto dq = h.n_runs ? heads_dq_kernel<D, BF16, true> : heads_dq_kernel<D, BF16, false>;
     EMMY_CUDA(cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<D>::kTotal));
     EMMY_CUDA(cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<D>::kTotal));
-    dkv<<<(unsigned)kv_ctas, kBwdThreads, BwdSmem<D>::kTotal, s>>>(mq, mk, mv, mdo, p);
+    dkv<<<(unsigned)kv_ctas, kBwdThreads, BwdSmem<D>::kTotal, s>>>(mq, mv_tile, mdo, p);
     rc = launch_status("heads_dkv_kernel");
     if (rc != EMMYB200_OK) return rc;
-    dq<<<(unsigned)q_ctas, kBwdThreads, BwdSmem<D>::kTotal, s>>>(mq, mk, mv, mdo, p);
+    dq<<<(unsigned)q_ctas, kBwdThreads, BwdSmem<D>::kTotal, s>>>(mk, mv, p);
     return launch_status("heads_dq_kernel");
 }
 
@@ -715,7 +782,7 @@ static int launch_bwd(BwdParams& p, cudaStream_t s) {
 
 bool heads_bwd_sm100_takes(const HeadsParams& p, int dtype, int d, const HeadsGrads& g) {
     using namespace heads;
-    return heads_sm100_takes(p, dtype, d, g.q, g.k, g.v, g.q) && map_fits(g.d_o, p.batch, p.heads, p.seq_q, p.do_s) &&
+    return heads_sm100_takes(p, dtype, d, g.q, g.k, g.v, g.o) && map_fits(g.d_o, p.batch, p.heads, p.seq_q, p.do_s) &&
            map_fits(g.dq, p.batch, p.heads, p.seq_q, p.dq_s) && map_fits(g.dk, p.batch, p.kv_heads, p.seq_k, p.dk_s) &&
            map_fits(g.dv, p.batch, p.kv_heads, p.seq_k, p.dv_s);
 }

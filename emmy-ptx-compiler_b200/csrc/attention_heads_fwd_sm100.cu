@@ -99,7 +99,7 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     float* xchg = reinterpret_cast<float*>(smem_gen + S::kXchgOffset);              // [2][2][128]
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int split = blockIdx.x % p.splits;
     const int item = blockIdx.x / p.splits;
     const int unit = item / p.tiles;
@@ -161,32 +161,36 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
         __syncwarp();
     } else if (warp == 1) {
-        // ---- MMA issuer ----------------------------------------------------------------------------------
-        if (lane == 0) {
+        // ---- MMA issuer: the whole warp, for its elected lane -----------------------------------------------
+        {
             constexpr uint32_t idesc_s = ptx::mma_idesc_f16(BF16, false, false, kTile, kTile);
             constexpr uint32_t idesc_o = ptx::mma_idesc_f16(BF16, false, true, kTile, D);
+            constexpr uint32_t hi = ptx::smem_desc_sw128_hi(1024);
+            const uint32_t lead = ptx::elect_lead();
             const uint32_t s_tmem = tmem_base, o_tmem = tmem_base + kColO;
-            bool ok = kv_tiles == 0 || bounded_wait(wctx, q_full, 0, 0x04030000u);
+            const uint32_t q_lo = ptx::smem_desc_sw128_lo(q_smem, 16), k_lo = ptx::smem_desc_sw128_lo(k_smem, 16), v_lo = ptx::smem_desc_sw128_lo(v_smem, kTile * 128);
+            auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) { return __all_sync(0xffffffffu, bounded_wait(wctx, bar, parity, code)) != 0; };
+            bool ok = kv_tiles == 0 || wait(q_full, 0, 0x04030000u);
             for (int j = 0; j < kv_tiles && ok; ++j) {
                 const uint32_t ph = j & 1;
-                if (!(ok = bounded_wait(wctx, k_full, ph, 0x04040000u | (j & 0xffff)))) break;
+                if (!(ok = wait(k_full, ph, 0x04040000u | (j & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {           // S = Q K^T, contraction over the head dim
-                    const uint32_t off = (kk / 4) * (kTile * 128) + (kk % 4) * 32;
-                    ptx::mma_ss(s_tmem, ptx::smem_desc_sw128(q_smem + off, 16, 1024), ptx::smem_desc_sw128(k_smem + off, 16, 1024), idesc_s, kk != 0);
+                    const uint32_t off = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) >> 4;
+                    ptx::mma_ss_lead(lead, s_tmem, q_lo + off, k_lo + off, hi, idesc_s, kk != 0);
                 }
-                ptx::mma_commit(k_empty);
-                ptx::mma_commit(s_full);
-                if (!(ok = bounded_wait(wctx, p_full, ph, 0x04050000u | (j & 0xffff)))) break;
-                if (!(ok = bounded_wait(wctx, v_full, ph, 0x04060000u | (j & 0xffff)))) break;
+                ptx::mma_commit_lead(lead, s_full);
+                ptx::mma_commit_lead(lead, k_empty);
+                if (!(ok = wait(p_full, ph, 0x04050000u | (j & 0xffff)))) break;
+                if (!(ok = wait(v_full, ph, 0x04060000u | (j & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
 #pragma unroll
                 for (int kk = 0; kk < kTile / 16; ++kk)         // O += P V, contraction over the keys
-                    ptx::mma_ts(o_tmem, s_tmem + kk * 8, ptx::smem_desc_sw128(v_smem + kk * (16 * 128), kTile * 128, 1024), idesc_o, (j | kk) != 0);
-                ptx::mma_commit(v_empty);
+                    ptx::mma_ts_lead(lead, o_tmem, s_tmem + kk * 8, v_lo + ((kk * 16 * 128) >> 4), hi, idesc_o, (j | kk) != 0);
+                ptx::mma_commit_lead(lead, v_empty);
             }
-            if (ok) ptx::mma_commit(o_full);
+            if (ok) ptx::mma_commit_lead(lead, o_full);
         }
         __syncwarp();
     } else {
