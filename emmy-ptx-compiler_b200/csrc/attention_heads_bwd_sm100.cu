@@ -13,13 +13,12 @@
 // do the arithmetic between them, taking the 64-column tiles in turn, one thread per row: while one group takes exponentials the products of
 // the other's tile run. Tensor memory (512 columns) sets the shape: with 128-column tiles there is room for one tile of S and dP
 // beside the accumulators, and a chain S -> exponentials -> P -> dV -> next S that left the tensor pipe idle for 40-58 % of the
-// time (measured: 3600 and 3790 cycles per 128 x 128 tile where the products take 2048 and 1536). With 64 columns S has two
-// buffers. In dkv a P tile (16 bits, 32 columns) goes back over the S tile it came from, dS beside it; in dq dS goes over dP,
-// so that the next S of a group is taken as soon as the last one is in registers.
-// A product with N = 64 would be bound by shared memory if both operands came from there (A is read again for every 64
-// columns: 48 cycles per 16-deep step against 32 of arithmetic), so the operand that stays, K in dkv, Q and dO in dq, is
-// written to tensor memory once and read from there; dkv has no room left for V.
-//   columns, dkv: S 2 x 64, dP 64, K 64, dV 128, dK 128      dq: S 2 x 64, dP 2 x 64, Q 64, dO 64, dQ 128
+// time (measured: 3600 and 3790 cycles per 128 x 128 tile where the products take 2048 and 1536). With 64 columns S and dP have two
+// buffers each. P (16 bits, 32 columns) goes back over the S tile it came from, dS over dP.
+// A product with N = 64 is bound by shared memory if both operands come from there (A is read again for every 64 columns: 48
+// cycles per 16-deep step against 32 with A in tensor memory), so where there is room the operand that stays is written to tensor memory
+// once and read from there: Q and dO in dq; K and V in dkv for d = 64.
+//   columns, dkv: S 2 x 64, dP 2 x 64, dV d, dK d (K 32, V 32)      dq: S 2 x 64, dP 2 x 64, Q d / 2, dO d / 2, dQ d
 //
 // Row terms come from the rows kernel already negated and shifted: nlse2 = -lse log2(e) + shift, -inf for rows that see
 // nothing or lie behind seq_q, so that P = 2^(scale log2(e) q.k + bias + nlse2) needs no test. The shift scales P by what the
@@ -52,9 +51,9 @@ constexpr int kHalf = 64;               // columns of a tile: rows of a stage
 template <int D>
 struct BwdSmem {
     static constexpr int kStage = kHalf * D * 2;
-    static constexpr int kStages = 5;                                   // dkv: of Q and of dO, beside the 128 rows of V
+    static constexpr int kStages = 4;                                   // dkv: of Q and of dO, beside 128 rows of K and V
     static constexpr int kStagesDq = 6;                                 // dq: of K and of V
-    static constexpr int kRing = 12 * kStage;                           // either way: 2 + 2 x 5, 2 x 6 stages
+    static constexpr int kRing = 12 * kStage;                           // either way: 4 + 2 x 4, 2 x 6 stages
     static constexpr int kRowsOffset = kRing;                           // dkv: [stage][nlse2 64, ndelta 64]
     static constexpr int kBarOffset = kRowsOffset + kStages * 512;
     static constexpr int kBiasOffset = kBarOffset + 512;
@@ -119,30 +118,25 @@ struct Products {
         for (int kk = 0; kk < kHalf / 16; ++kk) ptx::mma_ts_lead(lead, d, a + kk * 8, lo + ((kk * 16 * 128) >> 4), kHi, kGrads, !first || kk != 0);
     }
 };
-// A wait of the whole issuing warp: every lane polls, the answer is the warp's.
-__device__ __forceinline__ bool warp_spin(const WaitCtx& ctx, uint32_t bar, uint32_t parity, uint32_t code) {
-    return __all_sync(0xffffffffu, bounded_spin(ctx, bar, parity, code));
-}
-
 template <int D, bool BF16, bool BIAS>
 __global__ void __launch_bounds__(kBwdThreads, 1)
-heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
-                 const __grid_constant__ BwdParams p) {
+heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                 const __grid_constant__ CUtensorMap map_do, const __grid_constant__ BwdParams p) {
     using S = BwdSmem<D>;
     using Mma = Products<D, BF16>;
     constexpr int kChunks = D / 64, kStages = S::kStages;
-    constexpr uint32_t kColS = 0, kColDP = 128, kColK = 192, kColDV = 256, kColDK = 384;
+    constexpr bool kKvInTmem = D == 64;
+    constexpr uint32_t kColS = 0, kColDP = 128, kColDV = 256, kColDK = 256 + D, kColK = 384, kColV = 416;      // K and V: D = 64 only
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
-    const uint32_t v_smem = smem_base;
-    auto q_smem = [&](int s) { return smem_base + (2 + s) * S::kStage; };
-    auto do_smem = [&](int s) { return smem_base + (2 + kStages + s) * S::kStage; };
+    const uint32_t k_smem = smem_base, v_smem = smem_base + 2 * S::kStage;
+    auto q_smem = [&](int s) { return smem_base + (4 + s) * S::kStage; };
+    auto do_smem = [&](int s) { return smem_base + (4 + kStages + s) * S::kStage; };
     const uint32_t rows_smem = smem_base + S::kRowsOffset;
     const uint32_t bar_base = smem_base + S::kBarOffset;
-    const uint32_t k_ready = bar_base, v_full = bar_base + 8, acc_full = bar_base + 16, s_full = bar_base + 24 /* per group */, dp_full = bar_base + 40,
-                   p_ready = bar_base + 56, ds_ready = bar_base + 72, q_full = bar_base + 128, q_empty = q_full + 8 * kStages,
-                   do_full = q_empty + 8 * kStages, do_empty = do_full + 8 * kStages;
+    const uint32_t kv_ready = bar_base, acc_full = bar_base + 16, s_full = bar_base + 24 /* per group */, dp_full = bar_base + 40,
+                   p_ready = bar_base + 56, ds_ready = bar_base + 72, full = bar_base + 128, empty = full + 8 * kStages;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 96);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
@@ -159,17 +153,16 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
 
     if (threadIdx.x == 0) {
-        ptx::mbar_init(k_ready, 8); ptx::mbar_init(v_full, 1); ptx::mbar_init(acc_full, 1);
+        ptx::mbar_init(kv_ready, kKvInTmem ? 8 : 1); ptx::mbar_init(acc_full, 1);
         for (int x = 0; x < 2; ++x) {
             ptx::mbar_init(s_full + 8 * x, 1); ptx::mbar_init(dp_full + 8 * x, 1); ptx::mbar_init(p_ready + 8 * x, 4); ptx::mbar_init(ds_ready + 8 * x, 4);
         }
         for (int s = 0; s < kStages; ++s) {
-            ptx::mbar_init(q_full + 8 * s, 1); ptx::mbar_init(q_empty + 8 * s, 1);
-            ptx::mbar_init(do_full + 8 * s, 1); ptx::mbar_init(do_empty + 8 * s, 1);
+            ptx::mbar_init(full + 8 * s, 1); ptx::mbar_init(empty + 8 * s, 1);
         }
         *abort_flag = 0;
         ptx::mbar_fence_init();
-        ptx::prefetch_tensormap(&map_q); ptx::prefetch_tensormap(&map_v); ptx::prefetch_tensormap(&map_do);
+        ptx::prefetch_tensormap(&map_q); ptx::prefetch_tensormap(&map_k); ptx::prefetch_tensormap(&map_v); ptx::prefetch_tensormap(&map_do);
     }
     if (warp == 1) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
@@ -184,71 +177,70 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         // ---- TMA producer ------------------------------------------------------------------------------
         if (lane == 0 && n_it > 0) {
             int s = 0, gi = 0, qt = first_qt;
-            uint32_t empty = 1;
+            uint32_t phase = 1;
+            if (!kKvInTmem) {
+                ptx::mbar_arrive_expect_tx(kv_ready, 4 * S::kStage);
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    ptx::tma_load_4d(k_smem + c * (kTile * 128), &map_k, kv_ready, c * 64, key0, hk * p.k_at.head, b * p.k_at.batch);
+                    ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, kv_ready, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
+                }
+            }
             for (int it = 0; it < n_it; ++it) {
                 const int h = hk * p.h.group + gi, row0 = qt * kHalf;
-                if (!bounded_wait(wctx, q_empty + 8 * s, empty, 0x05010000u | (it & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(q_full + 8 * s, S::kStage + 512);
+                if (!bounded_wait(wctx, empty + 8 * s, phase, 0x05010000u | (it & 0xffff))) break;
+                ptx::mbar_arrive_expect_tx(full + 8 * s, 2 * S::kStage + 512);
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    ptx::tma_load_4d(q_smem(s) + c * Mma::kPiece, &map_q, q_full + 8 * s, c * 64, row0, h * p.q_at.head, b * p.q_at.batch);
-                const int64_t at = ((int64_t)b * p.h.heads + h) * p.g.pad_q + row0;
-                ptx::bulk_load(rows_smem + s * 512, p.g.lse2 + at, 256, q_full + 8 * s);
-                ptx::bulk_load(rows_smem + s * 512 + 256, p.g.delta + at, 256, q_full + 8 * s);
-                if (it == 0) {
-                    ptx::mbar_arrive_expect_tx(v_full, 2 * S::kStage);
-#pragma unroll
-                    for (int c = 0; c < kChunks; ++c)
-                        ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, v_full, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
+                for (int c = 0; c < kChunks; ++c) {
+                    ptx::tma_load_4d(q_smem(s) + c * Mma::kPiece, &map_q, full + 8 * s, c * 64, row0, h * p.q_at.head, b * p.q_at.batch);
+                    ptx::tma_load_4d(do_smem(s) + c * Mma::kPiece, &map_do, full + 8 * s, c * 64, row0, h * p.do_at.head, b * p.do_at.batch);
                 }
-                if (!bounded_wait(wctx, do_empty + 8 * s, empty, 0x05020000u | (it & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(do_full + 8 * s, S::kStage);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    ptx::tma_load_4d(do_smem(s) + c * Mma::kPiece, &map_do, do_full + 8 * s, c * 64, row0, h * p.do_at.head, b * p.do_at.batch);
-                if (++s == kStages) { s = 0; empty ^= 1; }
+                const int64_t at = ((int64_t)b * p.h.heads + h) * p.g.pad_q + row0;
+                ptx::bulk_load(rows_smem + s * 512, p.g.lse2 + at, 256, full + 8 * s);
+                ptx::bulk_load(rows_smem + s * 512 + 256, p.g.delta + at, 256, full + 8 * s);
+                if (++s == kStages) { s = 0; phase ^= 1; }
                 if (++qt == q_tiles) { qt = first_qt; ++gi; }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        // ---- MMA issuer: S(0) dP(0) S(1) | dV(i) dP(i+1) dK(i) S(i+2) | ... --------------------------------------
+        // ---- MMA issuer: S(0) dP(0) S(1) dP(1) | dV(i) S(i+2) dK(i) dP(i+2) | ... ----------------------------------
         if (n_it > 0) {
             const uint32_t lead = ptx::elect_lead();
-            int qs = 0, ds = 0;                                 // stages of the next S and of the next dP
-            uint32_t q_phase = 0, do_phase = 0;
-            auto s_product = [&](int it) {
-                if (!warp_spin(wctx, q_full + 8 * qs, q_phase, 0x05030000u | (it & 0xffff))) return false;
-                ptx::tc_fence_after_sync();
-                Mma::scores_ts(lead, tmem_base + kColS + 64 * (it & 1), tmem_base + kColK, q_smem(qs));
+            auto s_product = [&](int it, int s) {
+                if constexpr (kKvInTmem) Mma::scores_ts(lead, tmem_base + kColS + 64 * (it & 1), tmem_base + kColK, q_smem(s));
+                else Mma::scores_ss(lead, tmem_base + kColS + 64 * (it & 1), k_smem, q_smem(s));
                 ptx::mma_commit_lead(lead, s_full + 8 * (it & 1));
-                if (++qs == kStages) { qs = 0; q_phase ^= 1; }
-                return true;
             };
-            auto dp_product = [&](int it) {
-                if (!warp_spin(wctx, do_full + 8 * ds, do_phase, 0x05040000u | (it & 0xffff))) return false;
-                ptx::tc_fence_after_sync();
-                Mma::scores_ss(lead, tmem_base + kColDP, v_smem, do_smem(ds));
+            auto dp_product = [&](int it, int s) {
+                if constexpr (kKvInTmem) Mma::scores_ts(lead, tmem_base + kColDP + 64 * (it & 1), tmem_base + kColV, do_smem(s));
+                else Mma::scores_ss(lead, tmem_base + kColDP + 64 * (it & 1), v_smem, do_smem(s));
                 ptx::mma_commit_lead(lead, dp_full + 8 * (it & 1));
-                if (++ds == kStages) { ds = 0; do_phase ^= 1; }
-                return true;
             };
-            bool ok = warp_spin(wctx, k_ready, 0, 0x05050000u) && s_product(0) && warp_spin(wctx, v_full, 0, 0x05060000u) && dp_product(0);
-            if (ok && n_it > 1) ok = s_product(1);
-            int s = 0;
+            bool ok = warp_spin(wctx, kv_ready, 0, 0x05030000u);
+            for (int it = 0; it < 2 && it < n_it && ok; ++it) {
+                if (!(ok = warp_spin(wctx, full + 8 * it, 0, 0x05040000u | it))) break;
+                ptx::tc_fence_after_sync();
+                s_product(it, it);
+                dp_product(it, it);
+            }
+            int s = 0, next = 2;                                // stages of tiles it and it + 2
+            uint32_t next_phase = 0;
             for (int it = 0; it < n_it && ok; ++it) {
-                const uint32_t at = tmem_base + kColS + 64 * (it & 1), phase = (it >> 1) & 1;
+                const uint32_t x64 = 64 * (it & 1), phase = (it >> 1) & 1;
+                const bool more = it + 2 < n_it;
+                if (more && !(ok = warp_spin(wctx, full + 8 * next, next_phase, 0x05050000u | (it & 0xffff)))) break;
                 if (!(ok = warp_spin(wctx, p_ready + 8 * (it & 1), phase, 0x05070000u | (it & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
-                Mma::grads(lead, tmem_base + kColDV, at, do_smem(s), it == 0);
-                ptx::mma_commit_lead(lead, do_empty + 8 * s);
+                Mma::grads(lead, tmem_base + kColDV, tmem_base + kColS + x64, do_smem(s), it == 0);
+                if (more) s_product(it + 2, next);
                 if (!(ok = warp_spin(wctx, ds_ready + 8 * (it & 1), phase, 0x05080000u | (it & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
-                if (it + 1 < n_it && !(ok = dp_product(it + 1))) break;
-                Mma::grads(lead, tmem_base + kColDK, at + 32, q_smem(s), it == 0);
-                ptx::mma_commit_lead(lead, q_empty + 8 * s);
-                if (it + 2 < n_it && !(ok = s_product(it + 2))) break;
+                Mma::grads(lead, tmem_base + kColDK, tmem_base + kColDP + x64, q_smem(s), it == 0);
+                ptx::mma_commit_lead(lead, empty + 8 * s);
+                if (more) dp_product(it + 2, next);
                 if (++s == kStages) s = 0;
+                if (++next == kStages) { next = 0; next_phase ^= 1; }
             }
             if (ok) ptx::mma_commit_lead(lead, acc_full);
         }
@@ -257,15 +249,17 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         // ---- probabilities and their gradients: rows are keys, columns queries; group x takes tiles x, x + 2, ... ---------
         const int w = warp - 2, quarter = warp & 3, x = w >> 2;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        const uint32_t s_at = tmem_base + lane_base + kColS + x * 64, dp_at = tmem_base + lane_base + kColDP;
+        const uint32_t s_at = tmem_base + lane_base + kColS + x * 64, dp_at = tmem_base + lane_base + kColDP + x * 64;
         const int key = key0 + quarter * 32 + lane;
-        if (n_it > 0) {                                         // K into tensor memory, half of the head dim per group
-            row_to_tmem<D / 4>(tmem_base + lane_base + kColK + x * (D / 4),
-                               static_cast<const uint16_t*>(p.g.k) + b * p.h.k_s[0] + hk * p.h.k_s[1] + key * p.h.k_s[2] + x * (D / 2), key < n_keys);
+        if (kKvInTmem && n_it > 0) {                            // group 0 writes K to tensor memory, group 1 V
+            row_to_tmem<D / 2>(tmem_base + lane_base + (x ? kColV : kColK),
+                               x ? static_cast<const uint16_t*>(p.g.v) + b * p.h.v_s[0] + hk * p.h.v_s[1] + key * p.h.v_s[2]
+                                 : static_cast<const uint16_t*>(p.g.k) + b * p.h.k_s[0] + hk * p.h.k_s[1] + key * p.h.k_s[2],
+                               key < n_keys);
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(k_ready);
+            if (lane == 0) ptx::mbar_arrive(kv_ready);
         }
         const float g_scale = ds_scale<BF16>(p.g, bk, (int64_t)p.h.batch * p.h.kv_heads);
         const float2 g2 = make_float2(g_scale, g_scale);
@@ -277,7 +271,7 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
         int bias_head = -1;
         int gi = 0, qt = first_qt, s = x;                       // this group's tile and its stage
-        uint32_t q_phase = 0;
+        uint32_t full_phase = 0;
         if (x == 1 && ++qt == q_tiles) { qt = first_qt; ++gi; }
         for (int it = x; it < n_it && ok; it += 2) {
             const uint32_t phase = (it >> 1) & 1;
@@ -296,8 +290,7 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 looked_up = !wb.block(bias, value, w, lane, p.h.n_runs, key0 + quarter * 32 - (q0 + 63 + offset));
             }
-            ok = __all_sync(0xffffffffu, bounded_wait(wctx, q_full + 8 * s, q_phase, 0x050a0000u | (it & 0xffff)) &&
-                                             bounded_wait(wctx, s_full + 8 * x, phase, 0x050b0000u | (it & 0xffff)));
+            ok = warp_wait(wctx, full + 8 * s, full_phase, 0x050a0000u | (it & 0xffff)) && warp_wait(wctx, s_full + 8 * x, phase, 0x050b0000u | (it & 0xffff));
             if (!ok) break;
             ptx::tc_fence_after_sync();
             const float4* nlse = reinterpret_cast<const float4*>(smem_gen + S::kRowsOffset + s * 512);
@@ -349,7 +342,7 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(p_ready + 8 * x);
-            ok = __all_sync(0xffffffffu, bounded_wait(wctx, dp_full + 8 * x, phase, 0x050c0000u | (it & 0xffff)));
+            ok = warp_wait(wctx, dp_full + 8 * x, phase, 0x050c0000u | (it & 0xffff));
             if (!ok) break;
             ptx::tc_fence_after_sync();
             ptx::tmem_ld_32x32b_x32(dp_at, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
@@ -374,7 +367,7 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     pk[i - ch * 16] = operand_pair<BF16>(d0);
                     pk[i - ch * 16 + 1] = operand_pair<BF16>(d1);
                 }
-                ptx::tmem_st_32x32b_x16(s_at + 32 + ch * 16, pk);
+                ptx::tmem_st_32x32b_x16(dp_at + ch * 16, pk);
             }
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
@@ -382,12 +375,12 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             if (lane == 0) ptx::mbar_arrive(ds_ready + 8 * x);
             // two tiles on
             s += 2;
-            if (s >= kStages) { s -= kStages; q_phase ^= 1; }
+            if (s >= kStages) { s -= kStages; full_phase ^= 1; }
 #pragma unroll
             for (int k = 0; k < 2; ++k)
                 if (++qt == q_tiles) { qt = first_qt; ++gi; }
         }
-        if (ok && n_it > 0) ok = __all_sync(0xffffffffu, bounded_wait(wctx, acc_full, 0, 0x050d0000u));
+        if (ok && n_it > 0) ok = warp_wait(wctx, acc_full, 0, 0x050d0000u);
         if (ok) {                                               // group 0 writes dV, group 1 dK
             ptx::tc_fence_after_sync();
             const float f = (BF16 ? 1.0f : 1.0f / (1 << kF16Shift)) * (x ? p.h.scale / g_scale : 1.0f);
@@ -458,7 +451,7 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     auto v_smem = [&](int s) { return smem_base + (kStages + s) * S::kStage; };
     const uint32_t bar_base = smem_base + S::kBarOffset;
     const uint32_t a_ready = bar_base, acc_full = bar_base + 8, s_full = bar_base + 16 /* per group */, dp_full = bar_base + 32, ds_ready = bar_base + 48, s_free = bar_base + 64,
-                   k_full = bar_base + 128, k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages;
+                   full = bar_base + 128, empty = full + 8 * kStages;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 96);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
@@ -479,8 +472,7 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             ptx::mbar_init(s_full + 8 * x, 1); ptx::mbar_init(dp_full + 8 * x, 1); ptx::mbar_init(ds_ready + 8 * x, 4); ptx::mbar_init(s_free + 8 * x, 4);
         }
         for (int s = 0; s < kStages; ++s) {
-            ptx::mbar_init(k_full + 8 * s, 1); ptx::mbar_init(k_empty + 8 * s, 1);
-            ptx::mbar_init(v_full + 8 * s, 1); ptx::mbar_init(v_empty + 8 * s, 1);
+            ptx::mbar_init(full + 8 * s, 1); ptx::mbar_init(empty + 8 * s, 1);
         }
         *abort_flag = 0;
         ptx::mbar_fence_init();
@@ -500,20 +492,16 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         // ---- TMA producer ------------------------------------------------------------------------------
         if (lane == 0) {
             int s = 0;
-            uint32_t empty = 1;
+            uint32_t phase = 1;
             for (int it = 0; it < n_it; ++it) {
-                const int key0 = it * kHalf;
-                if (!bounded_wait(wctx, k_empty + 8 * s, empty, 0x06010000u | (it & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(k_full + 8 * s, S::kStage);
+                if (!bounded_wait(wctx, empty + 8 * s, phase, 0x06010000u | (it & 0xffff))) break;
+                ptx::mbar_arrive_expect_tx(full + 8 * s, 2 * S::kStage);
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    ptx::tma_load_4d(k_smem(s) + c * Mma::kPiece, &map_k, k_full + 8 * s, c * 64, key0, hk * p.k_at.head, b * p.k_at.batch);
-                if (!bounded_wait(wctx, v_empty + 8 * s, empty, 0x06020000u | (it & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(v_full + 8 * s, S::kStage);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    ptx::tma_load_4d(v_smem(s) + c * Mma::kPiece, &map_v, v_full + 8 * s, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
-                if (++s == kStages) { s = 0; empty ^= 1; }
+                for (int c = 0; c < kChunks; ++c) {
+                    ptx::tma_load_4d(k_smem(s) + c * Mma::kPiece, &map_k, full + 8 * s, c * 64, it * kHalf, hk * p.k_at.head, b * p.k_at.batch);
+                    ptx::tma_load_4d(v_smem(s) + c * Mma::kPiece, &map_v, full + 8 * s, c * 64, it * kHalf, hk * p.v_at.head, b * p.v_at.batch);
+                }
+                if (++s == kStages) { s = 0; phase ^= 1; }
             }
         }
         __syncwarp();
@@ -521,40 +509,40 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         // ---- MMA issuer: S(0) dP(0) S(1) dP(1) | S(i+2) dQ(i) dP(i+2) | ... ------------------------------------------
         if (n_it > 0) {
             const uint32_t lead = ptx::elect_lead();
-            int ks = 0, vs = 0;                                 // stages of the next S and of the next dP
-            uint32_t k_phase = 0, v_phase = 0;
-            auto s_product = [&](int it) {
-                if (!warp_spin(wctx, k_full + 8 * ks, k_phase, 0x06030000u | (it & 0xffff))) return false;
-                ptx::tc_fence_after_sync();
-                Mma::scores_ts(lead, tmem_base + kColS + 64 * (it & 1), tmem_base + kColQ, k_smem(ks));
+            auto s_product = [&](int it, int s) {
+                Mma::scores_ts(lead, tmem_base + kColS + 64 * (it & 1), tmem_base + kColQ, k_smem(s));
                 ptx::mma_commit_lead(lead, s_full + 8 * (it & 1));
-                if (++ks == kStages) { ks = 0; k_phase ^= 1; }
-                return true;
             };
-            auto dp_product = [&](int it) {
-                if (!warp_spin(wctx, v_full + 8 * vs, v_phase, 0x06040000u | (it & 0xffff))) return false;
-                ptx::tc_fence_after_sync();
-                Mma::scores_ts(lead, tmem_base + kColDP + 64 * (it & 1), tmem_base + kColDO, v_smem(vs));
+            auto dp_product = [&](int it, int s) {
+                Mma::scores_ts(lead, tmem_base + kColDP + 64 * (it & 1), tmem_base + kColDO, v_smem(s));
                 ptx::mma_commit_lead(lead, dp_full + 8 * (it & 1));
-                ptx::mma_commit_lead(lead, v_empty + 8 * vs);
-                if (++vs == kStages) { vs = 0; v_phase ^= 1; }
-                return true;
             };
-            bool ok = warp_spin(wctx, a_ready, 0, 0x06050000u) && s_product(0) && dp_product(0);
-            if (ok && n_it > 1) ok = s_product(1) && dp_product(1);
-            int s = 0;
+            bool ok = warp_spin(wctx, a_ready, 0, 0x06030000u);
+            for (int it = 0; it < 2 && it < n_it && ok; ++it) {
+                if (!(ok = warp_spin(wctx, full + 8 * it, 0, 0x06040000u | it))) break;
+                ptx::tc_fence_after_sync();
+                s_product(it, it);
+                dp_product(it, it);
+            }
+            int s = 0, next = 2;                                // stages of tiles it and it + 2
+            uint32_t next_phase = 0;
             for (int it = 0; it < n_it && ok; ++it) {
                 const uint32_t phase = (it >> 1) & 1;
-                if (it + 2 < n_it) {                            // S(it) is in registers: its columns are free
+                const bool more = it + 2 < n_it;
+                if (more) {
+                    if (!(ok = warp_spin(wctx, full + 8 * next, next_phase, 0x06050000u | (it & 0xffff)))) break;
+                    // S(it) is in registers: its columns are free
                     if (!(ok = warp_spin(wctx, s_free + 8 * (it & 1), phase, 0x06060000u | (it & 0xffff)))) break;
-                    if (!(ok = s_product(it + 2))) break;
+                    ptx::tc_fence_after_sync();
+                    s_product(it + 2, next);
                 }
                 if (!(ok = warp_spin(wctx, ds_ready + 8 * (it & 1), phase, 0x06070000u | (it & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
                 Mma::grads(lead, tmem_base + kColDQ, tmem_base + kColDP + 64 * (it & 1), k_smem(s), it == 0);
-                ptx::mma_commit_lead(lead, k_empty + 8 * s);
-                if (it + 2 < n_it && !(ok = dp_product(it + 2))) break;
+                ptx::mma_commit_lead(lead, empty + 8 * s);
+                if (more) dp_product(it + 2, next);
                 if (++s == kStages) s = 0;
+                if (++next == kStages) { next = 0; next_phase ^= 1; }
             }
             if (ok) ptx::mma_commit_lead(lead, acc_full);
         }
@@ -598,7 +586,7 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             float c = p.h.scale_log2, add = nlse;
             bool looked_up = false;
             if constexpr (BIAS) looked_up = !wb.block(bias, bias.value, w, lane, p.h.n_runs, d0);
-            ok = __all_sync(0xffffffffu, bounded_wait(wctx, s_full + 8 * x, phase, 0x06080000u | (it & 0xffff)));
+            ok = warp_wait(wctx, s_full + 8 * x, phase, 0x06080000u | (it & 0xffff));
             if (!ok) break;
             ptx::tc_fence_after_sync();
             const int valid = sees - key0;                      // columns that are seen
@@ -636,7 +624,7 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(k_smem(s) + ch * Mma::kPiece + k * 16), "r"(0) : "memory");
                 ptx::fence_proxy_async_smem();
             }
-            ok = __all_sync(0xffffffffu, bounded_wait(wctx, dp_full + 8 * x, phase, 0x06090000u | (it & 0xffff)));
+            ok = warp_wait(wctx, dp_full + 8 * x, phase, 0x06090000u | (it & 0xffff));
             if (!ok) break;
             ptx::tc_fence_after_sync();
             ptx::tmem_ld_32x32b_x32(dp_at, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
@@ -704,7 +692,7 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             s += 2;
             if (s >= kStages) s -= kStages;
         }
-        if (ok && n_it > 0) ok = __all_sync(0xffffffffu, bounded_wait(wctx, acc_full, 0, 0x060a0000u));
+        if (ok && n_it > 0) ok = warp_wait(wctx, acc_full, 0, 0x060a0000u);
         if (ok) {
             ptx::tc_fence_after_sync();
             const float out = BF16 ? 1.0f : 1.0f / ((1 << kF16Shift) * g_scale);
@@ -757,10 +745,11 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 template <int D, bool BF16>
 static int launch_bwd(BwdParams& p, cudaStream_t s) {
     const HeadsParams& h = p.h;
-    CUtensorMap mq, mk, mv, mv_tile, mdo;
+    CUtensorMap mq, mk, mv, mk_tile, mv_tile, mdo;
     int rc = make_map(&mq, &p.q_at, p.g.q, h.batch, h.heads, h.seq_q, D, h.q_s, kHalf, 1);
     if (rc == EMMYB200_OK) rc = make_map(&mk, &p.k_at, p.g.k, h.batch, h.kv_heads, h.seq_k, D, h.k_s, kHalf, 1);
     if (rc == EMMYB200_OK) rc = make_map(&mv, &p.v_at, p.g.v, h.batch, h.kv_heads, h.seq_k, D, h.v_s, kHalf, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&mk_tile, &p.k_at, p.g.k, h.batch, h.kv_heads, h.seq_k, D, h.k_s, kTile, 1);
     if (rc == EMMYB200_OK) rc = make_map(&mv_tile, &p.v_at, p.g.v, h.batch, h.kv_heads, h.seq_k, D, h.v_s, kTile, 1);
     if (rc == EMMYB200_OK) rc = make_map(&mdo, &p.do_at, p.g.d_o, h.batch, h.heads, h.seq_q, D, h.do_s, kHalf, 1);
     if (rc != EMMYB200_OK) return rc;
@@ -771,7 +760,7 @@ static int launch_bwd(BwdParams& p, cudaStream_t s) {
     auto dq = h.n_runs ? heads_dq_kernel<D, BF16, true> : heads_dq_kernel<D, BF16, false>;
     EMMY_CUDA(cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<D>::kTotal));
     EMMY_CUDA(cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<D>::kTotal));
-    dkv<<<(unsigned)kv_ctas, kBwdThreads, BwdSmem<D>::kTotal, s>>>(mq, mv_tile, mdo, p);
+    dkv<<<(unsigned)kv_ctas, kBwdThreads, BwdSmem<D>::kTotal, s>>>(mq, mk_tile, mv_tile, mdo, p);
     rc = launch_status("heads_dkv_kernel");
     if (rc != EMMYB200_OK) return rc;
     dq<<<(unsigned)q_ctas, kBwdThreads, BwdSmem<D>::kTotal, s>>>(mk, mv, p);
