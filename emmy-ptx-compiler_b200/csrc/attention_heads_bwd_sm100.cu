@@ -40,6 +40,7 @@ struct BwdParams {
     HeadsGrads g;
     MapAt q_at, k_at, v_at, do_at;
     int q_tiles, k_tiles;
+    int chunk_dkv, chunk_dq;            // of units, see work_item
     unsigned long long wait_limit_ns;
     uint32_t* status;
 };
@@ -58,7 +59,8 @@ struct BwdSmem {
     static constexpr int kBarOffset = kRowsOffset + kStages * 512;
     static constexpr int kBiasOffset = kBarOffset + 512;
     static constexpr int kSumsOffset = kBiasOffset + (int)sizeof(BiasShared);
-    static constexpr int kTotal = kSumsOffset + 8 * kHeadsMaxRuns * 4 + 1024;
+    static constexpr int kDiagOffset = kSumsOffset + 8 * kHeadsMaxRuns * 4;
+    static constexpr int kTotal = kDiagOffset + (int)sizeof(DiagShared) + 1024;
 };
 
 // The power of two dS is scaled by in f16: |dS| 2^14 g <= 2^15 from |dO . v - D| <= 2 max|dO| max|v|. 1 in bf16.
@@ -142,7 +144,8 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int kt = blockIdx.x % p.k_tiles, bk = blockIdx.x / p.k_tiles;         // causal: the first key tiles see the most queries
+    const WorkItem work = work_item(blockIdx.x, p.h.batch * p.h.kv_heads, p.k_tiles, p.chunk_dkv);
+    const int kt = work.tile, bk = work.unit;                   // causal: the first key tiles see the most queries
     const int b = bk / p.h.kv_heads, hk = bk % p.h.kv_heads;
     const int key0 = kt * kTile;
     const int n_keys = heads_key_count(p.h, b), offset = heads_offset(p.h, n_keys);
@@ -422,9 +425,11 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 }
 
 // The gradient of the bias, one warp's share: 32 x 64 blocks of dS. A block inside one run adds to a per-thread sum, which goes
-// to the warp's sum of that run when the run changes; other blocks are added up along their 95 diagonals. Diagonal sums need
-// no atomics: a partial sum moves one lane up per column, so that it follows its diagonal and is complete when it reaches lane 31
-// (or the last column); every step adds one column of all 32 diagonals that pass it.
+// to the warp's sum of that run when the run changes; other blocks are added up along their 95 diagonals, without atomics: a partial
+// sum moves one lane up per column, so that it follows its diagonal and is complete when it reaches lane 31. Four chains of 16 columns run side by
+// side (one of 64 was bound by the shuffle's latency: 55 us of dq for 96 units of 512 x 512 x 64, 8 tiles each); what the lanes hold
+// after a chain's last column are partial sums of the 32 diagonals that go on into the next. Each run the block touches is then
+// added up by one lane, whole groups of eight diagonals at a time.
 struct RunSums {
     float acc;              // this thread's part of the run
     int run;
@@ -455,10 +460,11 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 96);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
+    DiagShared& diag = *reinterpret_cast<DiagShared*>(smem_gen + S::kDiagOffset);
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int bh = blockIdx.x / p.q_tiles;
-    const int qt = p.h.causal ? p.q_tiles - 1 - (int)(blockIdx.x % p.q_tiles) : (int)(blockIdx.x % p.q_tiles);
+    const WorkItem work = work_item(blockIdx.x, p.h.batch * p.h.heads, p.q_tiles, p.chunk_dq);
+    const int bh = work.unit, qt = p.h.causal ? p.q_tiles - 1 - work.tile : work.tile;
     const int b = bh / p.h.heads, h = bh % p.h.heads, hk = h / p.h.group;
     const int row0 = qt * kTile;
     const int n_keys = heads_key_count(p.h, b), offset = heads_offset(p.h, n_keys);
@@ -656,22 +662,53 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             if (lane == 0) ptx::mbar_arrive(ds_ready + 8 * x);
             if constexpr (BIAS) {
                 if (want_bias) {
-                    if (looked_up) {                            // the biases have been read: the diagonal sums take their place
-                        float diag = 0.0f;                      // a diagonal's partial sum, passing through this lane
+                    if (looked_up) {
+                        const float go_on = lane == 0 ? 0.0f : 1.0f;
 #pragma unroll
-                        for (int i = 0; i < 64; ++i) {
-                            const float below = __shfl_up_sync(0xffffffffu, diag, 1);
-                            diag = (lane == 0 ? 0.0f : below) + __uint_as_float(r[i]);
-                            if (lane == 31) bias.by_dist[w][i] = diag;
+                        for (int i = 1; i < 16; ++i)
+#pragma unroll
+                            for (int chain = 0; chain < 64; chain += 16) {
+                                const float below = __shfl_up_sync(0xffffffffu, __uint_as_float(r[chain + i - 1]), 1);
+                                r[chain + i] = __float_as_uint(fmaf(below, go_on, __uint_as_float(r[chain + i])));
+                            }
+                        if (lane == 31) {
+#pragma unroll
+                            for (int i = 0; i < 64; i += 4) *reinterpret_cast<uint4*>(&diag.complete[w][i]) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
                         }
-                        if (lane < 31) bias.by_dist[w][94 - lane] = diag;
+#pragma unroll
+                        for (int chain = 0; chain < 4; ++chain) diag.rest[w][chain][lane] = lane == 31 ? 0.0f : __uint_as_float(r[16 * chain + 15]);
+                        __syncwarp();
+                        // lane: diagonals 3 lane .. 3 lane + 2; lane l's rest of chain c belongs to diagonal 16 c + 46 - l
+                        float d3[3];
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) {
+                            const int t = 3 * lane + k;
+                            d3[k] = t < 64 ? diag.complete[w][t] : 0.0f;
+#pragma unroll
+                            for (int chain = 0; chain < 4; ++chain) {
+                                const int from = 16 * chain + 46 - t;
+                                if (from >= 0 && from < 32) d3[k] += diag.rest[w][chain][from];
+                            }
+                        }
+                        float* by_diag = bias.by_dist[w];                   // the biases have been read
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) by_diag[3 * lane + k] = d3[k];
+                        __syncwarp();
+                        float* eights = diag.rest[w][0];                    // sums of eight neighbours
+                        if (lane < 12) {
+                            const float4 lo = *reinterpret_cast<const float4*>(by_diag + 8 * lane), hi = *reinterpret_cast<const float4*>(by_diag + 8 * lane + 4);
+                            eights[lane] = ((lo.x + lo.y) + (lo.z + lo.w)) + ((hi.x + hi.y) + (hi.z + hi.w));
+                        }
                         __syncwarp();
                         // runs the block touches, one lane each
                         const int ra = heads_run_of(bias.first, p.h.n_runs, d0), rb = heads_run_of(bias.first, p.h.n_runs, d0 + 94);
                         for (int run = ra + lane; run <= rb; run += 32) {
-                            const int from = run == ra ? 0 : bias.first[run] - d0, to = run == rb ? 95 : bias.first[run + 1] - d0;
+                            int t = run == ra ? 0 : bias.first[run] - d0;
+                            const int to = run == rb ? 95 : bias.first[run + 1] - d0;
                             float v = 0.0f;
-                            for (int t = from; t < to; ++t) v += bias.by_dist[w][t];
+                            for (; t < to && (t & 7) != 0; ++t) v += by_diag[t];
+                            for (; t + 8 <= to; t += 8) v += eights[t >> 3];
+                            for (; t < to; ++t) v += by_diag[t];
                             sums[run] += v;
                         }
                         __syncwarp();
@@ -756,6 +793,8 @@ static int launch_bwd(BwdParams& p, cudaStream_t s) {
     EMMY_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p.status), g_bwd_status));
     const int64_t kv_ctas = (int64_t)h.batch * h.kv_heads * p.k_tiles, q_ctas = (int64_t)h.batch * h.heads * p.q_tiles;
     if (kv_ctas >= (1ll << 31) || q_ctas >= (1ll << 31)) return fail(EMMYB200_ERR_SHAPE, "attention_heads_bwd: the tiles exceed the grid limit");
+    p.chunk_dkv = chunk_units(h.causal != 0, (int64_t)h.batch * h.kv_heads, (int64_t)h.seq_q * D * 4 * h.group);
+    p.chunk_dq = chunk_units(h.causal != 0, (int64_t)h.batch * h.heads, (int64_t)h.seq_k * D * 4 / h.group);
     auto dkv = h.n_runs ? heads_dkv_kernel<D, BF16, true> : heads_dkv_kernel<D, BF16, false>;
     auto dq = h.n_runs ? heads_dq_kernel<D, BF16, true> : heads_dq_kernel<D, BF16, false>;
     EMMY_CUDA(cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<D>::kTotal));

@@ -30,6 +30,7 @@ struct FwdParams {
     MapAt q_at, k_at, v_at, o_at;
     int packed;                         // rows of a tile: group x seq_q (1) or 128 queries of one head (0)
     int tiles;                          // query tiles per unit (batch entry and head, or key head when packed)
+    int chunk;                          // of units, see work_item
     int splits;                         // CTAs that share a tile's keys
     float* lse;
     float* part_o;                      // splits > 1: [split][row][D], rows as lse
@@ -102,10 +103,9 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int split = blockIdx.x % p.splits;
     const int item = blockIdx.x / p.splits;
-    const int unit = item / p.tiles;
-    // causal tiles differ in length: the longest of each unit first
-    const int qt = p.h.causal ? p.tiles - 1 - item % p.tiles : item % p.tiles;
     const int unit_heads = p.packed ? p.h.kv_heads : p.h.heads;
+    const WorkItem work = work_item(item, p.h.batch * unit_heads, p.tiles, p.chunk);
+    const int unit = work.unit, qt = p.h.causal ? p.tiles - 1 - work.tile : work.tile;
     const int b = unit / unit_heads, hu = unit % unit_heads;
     const int head0 = p.packed ? hu * p.h.group : hu, hk = p.packed ? hu : hu / p.h.group;
     const int row0 = qt * kTile;
@@ -428,6 +428,7 @@ static int launch(FwdParams& p, const FwdPlan& plan, const void* Q, const void* 
     EMMY_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p.status), g_fwd_status));
     const int64_t ctas = (int64_t)p.h.batch * (plan.packed ? p.h.kv_heads : p.h.heads) * p.tiles * p.splits;
     if (ctas >= (1ll << 31)) return fail(EMMYB200_ERR_SHAPE, "attention_heads_fwd: %lld tiles exceed the grid limit", (long long)ctas);
+    p.chunk = chunk_units(p.h.causal != 0, (int64_t)p.h.batch * (plan.packed ? p.h.kv_heads : p.h.heads), (int64_t)p.h.seq_k * D * 4 / (plan.packed ? 1 : p.h.group));
     auto kernel = p.h.n_runs ? heads_fwd_kernel<D, BF16, true> : heads_fwd_kernel<D, BF16, false>;
     EMMY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdSmem<D>::kTotal));
     kernel<<<(unsigned)ctas, kFwdThreads, FwdSmem<D>::kTotal, s>>>(mq, mk, mv, mo, p);

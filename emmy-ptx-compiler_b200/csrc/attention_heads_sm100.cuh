@@ -3,6 +3,7 @@
 // operands.
 #pragma once
 #include <limits.h>
+#include <stddef.h>
 
 #include "attention_heads.cuh"
 #include "sm100_ptx.cuh"
@@ -97,6 +98,12 @@ struct BiasShared {
     float value[kHeadsMaxRuns];         // of the head, log2 units
     float by_dist[8][96];               // one row per warp
 };
+static_assert(offsetof(BiasShared, by_dist) % 16 == 0, "read as float4");
+// dq: sums along the diagonals of a warp's block of dS
+struct DiagShared {
+    float complete[8][64];              // what lane 31 saw: by column
+    float rest[8][4][32];               // what the lanes were left with after columns 15, 31, 47, 63
+};
 struct WarpBias {
     int lo, hi;                         // distances [lo, hi) have the bias `same`
     int run;                            // its run
@@ -128,6 +135,26 @@ __device__ __forceinline__ void load_bias(BiasShared& s, const HeadsParams& p, i
         s.first[r] = p.run_first[r];
         s.value[r] = heads_run_bias(p, r, head);
     }
+}
+
+// ---- the order of the work items -----------------------------------------------------------------------------------------------
+// Causal tiles differ in length. Dealt longest first over many units the SMs finish together; dealt unit by unit the last units'
+// longest tiles run alone (16 units of 2048 keys on 148 SMs: 184 us against 118). But CTAs that run at the same time should share
+// what they stream, so the units are taken in chunks whose streamed operands fit in a third of L2, each chunk longest first. chunk = 1: unit by
+// unit (tiles of equal length).
+struct WorkItem {
+    int unit, tile;                     // tile: 0 is the longest
+};
+__device__ __forceinline__ WorkItem work_item(int item, int units, int tiles, int chunk) {
+    const int c = item / (chunk * tiles), in_chunk = item - c * chunk * tiles;
+    const int width = min(chunk, units - c * chunk);
+    return {c * chunk + in_chunk % width, in_chunk / width};
+}
+// `bytes`: streamed by one unit's tiles.
+inline int chunk_units(bool causal, int64_t units, int64_t bytes) {
+    if (!causal) return 1;
+    const int64_t fit = (42ll << 20) / (bytes > 0 ? bytes : 1);
+    return (int)(fit < 1 ? 1 : fit > units ? units : fit);
 }
 
 // ---- strided operands ---------------------------------------------------------------------------------------------------

@@ -7,7 +7,6 @@ path: without the library, or without a CUDA device, every call raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from pathlib import Path
@@ -683,16 +682,42 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-@contextlib.contextmanager
-def _on(device, stream):
+class _On:
     """The tensors' device and the launch's stream made current: what is allocated inside belongs to that stream."""
+
+    def __init__(self, device, stream) -> None:
+        self.device, self.stream = device, stream
+
+    def __enter__(self) -> int:
+        import torch
+        self.guards = [torch.cuda.device(self.device)] + ([torch.cuda.stream(self.stream)] if self.stream is not None else [])
+        for g in self.guards:
+            g.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *error) -> None:
+        for g in reversed(self.guards):
+            g.__exit__(*error)
+
+
+class _OnCurrent:
+    """The same where both are current already: nothing to switch."""
+
+    def __init__(self, handle: int) -> None:
+        self.handle = handle
+
+    def __enter__(self) -> int:
+        return self.handle
+
+    def __exit__(self, *error) -> None:
+        pass
+
+
+def _on(device, stream):
     import torch
-    with torch.cuda.device(device):
-        if stream is None:
-            yield torch.cuda.current_stream().cuda_stream
-        else:
-            with torch.cuda.stream(stream):
-                yield stream.cuda_stream
+    if stream is None and torch.cuda.current_device() == device.index:
+        return _OnCurrent(torch.cuda.current_stream(device.index).cuda_stream)
+    return _On(device, stream)
 
 
 def _heads_workspace(who: str, workspace, need: int, device):
