@@ -72,13 +72,15 @@ __device__ __forceinline__ float ds_scale(const HeadsGrads& g, int64_t bk, int64
     return __int_as_float(((int)fminf(fmaxf(floorf(-log2f(bound)), -100.0f), 100.0f) + 127) << 23);
 }
 
-// A row of a strided operand into tensor memory, as the A operand of a product: element pairs in columns. Rows that do not
-// exist are zeros. `cols` tensor-memory columns (two elements each) from `src`.
+// A row of a strided operand on its way into tensor memory, as the A operand of a product: element pairs in columns, COLS of
+// them. Loaded before the CTA has its tensor memory, stored after. Rows that do not exist are zeros.
 template <int COLS>
-__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const uint16_t* src, bool exists) {
-    uint4 v[COLS / 4];
+__device__ __forceinline__ void load_row(uint4 (&v)[COLS / 4], const uint16_t* src, bool exists) {
 #pragma unroll
     for (int i = 0; i < COLS / 4; ++i) v[i] = exists ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+}
+template <int COLS>
+__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const uint4 (&v)[COLS / 4]) {
 #pragma unroll
     for (int i = 0; i < COLS / 16; ++i) {
         uint32_t r[16];
@@ -155,6 +157,25 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const int n_it = per_head * p.h.group;
     const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
 
+    auto load_stage = [&](int s, int gi, int qt) {
+        const int h = hk * p.h.group + gi, row0 = qt * kHalf;
+        ptx::mbar_arrive_expect_tx(full + 8 * s, 2 * S::kStage + 512);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            ptx::tma_load_4d(q_smem(s) + c * Mma::kPiece, &map_q, full + 8 * s, c * 64, row0, h * p.q_at.head, b * p.q_at.batch);
+            ptx::tma_load_4d(do_smem(s) + c * Mma::kPiece, &map_do, full + 8 * s, c * 64, row0, h * p.do_at.head, b * p.do_at.batch);
+        }
+        const int64_t at = ((int64_t)b * p.h.heads + h) * p.g.pad_q + row0;
+        ptx::bulk_load(rows_smem + s * 512, p.g.lse2 + at, 256, full + 8 * s);
+        ptx::bulk_load(rows_smem + s * 512 + 256, p.g.delta + at, 256, full + 8 * s);
+    };
+    int load_it = 0, load_gi = 0, load_qt = first_qt, load_s = 0;               // the producer's next tile and stage
+    uint32_t load_phase = 1;
+    auto advance = [&]() {
+        if (++load_s == kStages) { load_s = 0; load_phase ^= 1; }
+        if (++load_qt == q_tiles) { load_qt = first_qt; ++load_gi; }
+        ++load_it;
+    };
     if (threadIdx.x == 0) {
         ptx::mbar_init(kv_ready, kKvInTmem ? 8 : 1); ptx::mbar_init(acc_full, 1);
         for (int x = 0; x < 2; ++x) {
@@ -165,8 +186,30 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
         *abort_flag = 0;
         ptx::mbar_fence_init();
-        ptx::prefetch_tensormap(&map_q); ptx::prefetch_tensormap(&map_k); ptx::prefetch_tensormap(&map_v); ptx::prefetch_tensormap(&map_do);
+        if (n_it > 0) {                                         // the first loads fly while the CTA sets itself up
+            if (!kKvInTmem) {
+                ptx::mbar_arrive_expect_tx(kv_ready, 4 * S::kStage);
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    ptx::tma_load_4d(k_smem + c * (kTile * 128), &map_k, kv_ready, c * 64, key0, hk * p.k_at.head, b * p.k_at.batch);
+                    ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, kv_ready, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
+                }
+            }
+            for (; load_it < n_it && load_it < kStages; advance()) load_stage(load_s, load_gi, load_qt);
+        }
     }
+    const int x = (warp - 2) >> 2;                              // group of the warps 2 to 9
+    const int key = key0 + (warp & 3) * 32 + lane;
+    uint4 a_row[D / 8];
+    float g_scale = 1.0f;
+    if (warp >= 2 && n_it > 0) {
+        if constexpr (kKvInTmem)                                // group 0 brings K to tensor memory, group 1 V
+            load_row<D / 2>(a_row, x ? static_cast<const uint16_t*>(p.g.v) + b * p.h.v_s[0] + hk * p.h.v_s[1] + key * p.h.v_s[2]
+                                     : static_cast<const uint16_t*>(p.g.k) + b * p.h.k_s[0] + hk * p.h.k_s[1] + key * p.h.k_s[2],
+                            key < n_keys);
+        g_scale = ds_scale<BF16>(p.g, bk, (int64_t)p.h.batch * p.h.kv_heads);
+    }
+    if constexpr (BIAS) load_runs(bias, p.h, warp, kBwdThreads / 32, lane);
     if (warp == 1) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
         ptx::tmem_relinquish();
@@ -178,31 +221,10 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 
     if (warp == 0) {
         // ---- TMA producer ------------------------------------------------------------------------------
-        if (lane == 0 && n_it > 0) {
-            int s = 0, gi = 0, qt = first_qt;
-            uint32_t phase = 1;
-            if (!kKvInTmem) {
-                ptx::mbar_arrive_expect_tx(kv_ready, 4 * S::kStage);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c) {
-                    ptx::tma_load_4d(k_smem + c * (kTile * 128), &map_k, kv_ready, c * 64, key0, hk * p.k_at.head, b * p.k_at.batch);
-                    ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, kv_ready, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
-                }
-            }
-            for (int it = 0; it < n_it; ++it) {
-                const int h = hk * p.h.group + gi, row0 = qt * kHalf;
-                if (!bounded_wait(wctx, empty + 8 * s, phase, 0x05010000u | (it & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(full + 8 * s, 2 * S::kStage + 512);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c) {
-                    ptx::tma_load_4d(q_smem(s) + c * Mma::kPiece, &map_q, full + 8 * s, c * 64, row0, h * p.q_at.head, b * p.q_at.batch);
-                    ptx::tma_load_4d(do_smem(s) + c * Mma::kPiece, &map_do, full + 8 * s, c * 64, row0, h * p.do_at.head, b * p.do_at.batch);
-                }
-                const int64_t at = ((int64_t)b * p.h.heads + h) * p.g.pad_q + row0;
-                ptx::bulk_load(rows_smem + s * 512, p.g.lse2 + at, 256, full + 8 * s);
-                ptx::bulk_load(rows_smem + s * 512 + 256, p.g.delta + at, 256, full + 8 * s);
-                if (++s == kStages) { s = 0; phase ^= 1; }
-                if (++qt == q_tiles) { qt = first_qt; ++gi; }
+        if (lane == 0) {
+            for (; load_it < n_it; advance()) {
+                if (!bounded_wait(wctx, empty + 8 * load_s, load_phase, 0x05010000u | (load_it & 0xffff))) break;
+                load_stage(load_s, load_gi, load_qt);
             }
         }
         __syncwarp();
@@ -250,28 +272,20 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         __syncwarp();
     } else {
         // ---- probabilities and their gradients: rows are keys, columns queries; group x takes tiles x, x + 2, ... ---------
-        const int w = warp - 2, quarter = warp & 3, x = w >> 2;
+        const int w = warp - 2, quarter = warp & 3;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_at = tmem_base + lane_base + kColS + x * 64, dp_at = tmem_base + lane_base + kColDP + x * 64;
-        const int key = key0 + quarter * 32 + lane;
-        if (kKvInTmem && n_it > 0) {                            // group 0 writes K to tensor memory, group 1 V
-            row_to_tmem<D / 2>(tmem_base + lane_base + (x ? kColV : kColK),
-                               x ? static_cast<const uint16_t*>(p.g.v) + b * p.h.v_s[0] + hk * p.h.v_s[1] + key * p.h.v_s[2]
-                                 : static_cast<const uint16_t*>(p.g.k) + b * p.h.k_s[0] + hk * p.h.k_s[1] + key * p.h.k_s[2],
-                               key < n_keys);
+        if (kKvInTmem && n_it > 0) {
+            row_to_tmem<D / 2>(tmem_base + lane_base + (x ? kColV : kColK), a_row);
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(kv_ready);
         }
-        const float g_scale = ds_scale<BF16>(p.g, bk, (int64_t)p.h.batch * p.h.kv_heads);
         const float2 g2 = make_float2(g_scale, g_scale);
         bool ok = true;
-        WarpBias wb;
+        WarpBias wb(p.h);
         float* value = reinterpret_cast<float*>(smem_gen + S::kSumsOffset) + w * kHeadsMaxRuns;
-        if constexpr (BIAS) {
-            for (int r = lane; r < p.h.n_runs; r += 32) bias.first[r] = p.h.run_first[r];       // every warp writes the same
-        }
         int bias_head = -1;
         int gi = 0, qt = first_qt, s = x;                       // this group's tile and its stage
         uint32_t full_phase = 0;
@@ -472,6 +486,14 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     const int n_it = (key_end + kHalf - 1) / kHalf;
     const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
 
+    auto load_stage = [&](int s, int it) {
+        ptx::mbar_arrive_expect_tx(full + 8 * s, 2 * S::kStage);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            ptx::tma_load_4d(k_smem(s) + c * Mma::kPiece, &map_k, full + 8 * s, c * 64, it * kHalf, hk * p.k_at.head, b * p.k_at.batch);
+            ptx::tma_load_4d(v_smem(s) + c * Mma::kPiece, &map_v, full + 8 * s, c * 64, it * kHalf, hk * p.v_at.head, b * p.v_at.batch);
+        }
+    };
     if (threadIdx.x == 0) {
         ptx::mbar_init(a_ready, 8); ptx::mbar_init(acc_full, 1);
         for (int x = 0; x < 2; ++x) {
@@ -482,9 +504,25 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
         *abort_flag = 0;
         ptx::mbar_fence_init();
-        ptx::prefetch_tensormap(&map_k); ptx::prefetch_tensormap(&map_v);
+        for (int it = 0; it < n_it && it < kStages; ++it) load_stage(it, it);           // these loads fly while the CTA sets itself up
     }
-    if (BIAS) load_bias(bias, p.h, h, threadIdx.x, kBwdThreads);
+    const int x = (warp - 2) >> 2;                              // group of the warps 2 to 9
+    const int row = row0 + (warp & 3) * 32 + lane;
+    uint4 a_row[D / 8];
+    float nlse = 0.0f, ndelta = 0.0f, g_scale = 1.0f;
+    if (warp >= 2) {                                            // group 0 brings Q to tensor memory, group 1 dO
+        load_row<D / 2>(a_row, x ? static_cast<const uint16_t*>(p.g.d_o) + b * p.h.do_s[0] + h * p.h.do_s[1] + row * p.h.do_s[2]
+                                 : static_cast<const uint16_t*>(p.g.q) + b * p.h.q_s[0] + h * p.h.q_s[1] + row * p.h.q_s[2],
+                        row < p.h.seq_q);
+        const int64_t at_row = (int64_t)bh * p.g.pad_q + row;
+        nlse = p.g.lse2[at_row];
+        ndelta = p.g.delta[at_row];
+        g_scale = ds_scale<BF16>(p.g, b * p.h.kv_heads + hk, (int64_t)p.h.batch * p.h.kv_heads);
+    }
+    if constexpr (BIAS) {
+        load_runs(bias, p.h, warp, kBwdThreads / 32, lane);
+        for (int r = threadIdx.x; r < p.h.n_runs; r += kBwdThreads) bias.value[r] = heads_run_bias(p.h, r, h);
+    }
     if (warp == 1) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
         ptx::tmem_relinquish();
@@ -498,15 +536,10 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         // ---- TMA producer ------------------------------------------------------------------------------
         if (lane == 0) {
             int s = 0;
-            uint32_t phase = 1;
-            for (int it = 0; it < n_it; ++it) {
+            uint32_t phase = 0;                                 // of the first release
+            for (int it = kStages; it < n_it; ++it) {
                 if (!bounded_wait(wctx, empty + 8 * s, phase, 0x06010000u | (it & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(full + 8 * s, 2 * S::kStage);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c) {
-                    ptx::tma_load_4d(k_smem(s) + c * Mma::kPiece, &map_k, full + 8 * s, c * 64, it * kHalf, hk * p.k_at.head, b * p.k_at.batch);
-                    ptx::tma_load_4d(v_smem(s) + c * Mma::kPiece, &map_v, full + 8 * s, c * 64, it * kHalf, hk * p.v_at.head, b * p.v_at.batch);
-                }
+                load_stage(s, it);
                 if (++s == kStages) { s = 0; phase ^= 1; }
             }
         }
@@ -555,31 +588,23 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         __syncwarp();
     } else {
         // ---- probabilities and their gradients: rows are queries, columns keys; group x takes tiles x, x + 2, ... --------
-        const int w = warp - 2, quarter = warp & 3, x = w >> 2;
+        const int w = warp - 2, quarter = warp & 3;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_at = tmem_base + lane_base + kColS + x * 64, dp_at = tmem_base + lane_base + kColDP + x * 64;
-        const int row = row0 + quarter * 32 + lane;
-        if (n_it > 0) {                                         // group 0 writes Q to tensor memory, group 1 dO
-            row_to_tmem<D / 2>(tmem_base + lane_base + (x ? kColDO : kColQ),
-                               x ? static_cast<const uint16_t*>(p.g.d_o) + b * p.h.do_s[0] + h * p.h.do_s[1] + row * p.h.do_s[2]
-                                 : static_cast<const uint16_t*>(p.g.q) + b * p.h.q_s[0] + h * p.h.q_s[1] + row * p.h.q_s[2],
-                               row < p.h.seq_q);
+        if (n_it > 0) {
+            row_to_tmem<D / 2>(tmem_base + lane_base + (x ? kColDO : kColQ), a_row);
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(a_ready);
         }
-        const int64_t at_row = (int64_t)bh * p.g.pad_q + row;
-        const float nlse = p.g.lse2[at_row], ndelta = p.g.delta[at_row];
-        const float g_scale = ds_scale<BF16>(p.g, b * p.h.kv_heads + hk, (int64_t)p.h.batch * p.h.kv_heads);
         const float2 nd2 = make_float2(ndelta, ndelta), g2 = make_float2(g_scale, g_scale);
         const int sees = p.h.causal ? min(n_keys, row + offset + 1) : n_keys;
         const bool want_bias = BIAS && p.g.dtable != nullptr;
         float* sums = reinterpret_cast<float*>(smem_gen + S::kSumsOffset) + w * kHeadsMaxRuns;      // this warp's, by run
         RunSums rs{0.0f, 0};
         bool ok = true;
-        WarpBias wb;
-        wb.reset();
+        WarpBias wb(p.h);
         if constexpr (BIAS) {
             for (int r = lane; r < p.h.n_runs; r += 32) sums[r] = 0.0f;
             __syncwarp();
@@ -701,7 +726,7 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                         }
                         __syncwarp();
                         // runs the block touches, one lane each
-                        const int ra = heads_run_of(bias.first, p.h.n_runs, d0), rb = heads_run_of(bias.first, p.h.n_runs, d0 + 94);
+                        const int ra = wb.run_of(bias, p.h.n_runs, d0), rb = wb.run_of(bias, p.h.n_runs, d0 + 94);
                         for (int run = ra + lane; run <= rb; run += 32) {
                             int t = run == ra ? 0 : bias.first[run] - d0;
                             const int to = run == rb ? 95 : bias.first[run + 1] - d0;

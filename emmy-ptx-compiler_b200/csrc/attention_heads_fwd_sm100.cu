@@ -118,6 +118,18 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const int kv_tiles = (int)((long long)all_tiles * (split + 1) / p.splits) - tile_first;
     const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
 
+    auto load_k = [&](int j) {
+        ptx::mbar_arrive_expect_tx(k_full, S::kOperand);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+            ptx::tma_load_4d(k_smem + c * (kTile * 128), &map_k, k_full, c * 64, (tile_first + j) * kTile, hk * p.k_at.head, b * p.k_at.batch);
+    };
+    auto load_v = [&](int j) {
+        ptx::mbar_arrive_expect_tx(v_full, S::kOperand);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+            ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, v_full, c * 64, (tile_first + j) * kTile, hk * p.v_at.head, b * p.v_at.batch);
+    };
     if (threadIdx.x == 0) {
         ptx::mbar_init(q_full, 1); ptx::mbar_init(k_full, 1); ptx::mbar_init(v_full, 1);
         ptx::mbar_init(k_empty, 1); ptx::mbar_init(v_empty, 1);
@@ -125,9 +137,19 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         for (int q = 0; q < 16; ++q) pair_flags[q] = 0;
         *abort_flag = 0;
         ptx::mbar_fence_init();
-        ptx::prefetch_tensormap(&map_q); ptx::prefetch_tensormap(&map_k); ptx::prefetch_tensormap(&map_v);
+        if (kv_tiles > 0) {                                     // the first loads fly while the CTA sets itself up
+            ptx::mbar_arrive_expect_tx(q_full, box_rows * D * 2);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+                ptx::tma_load_4d(q_smem + c * (kTile * 128), &map_q, q_full, c * 64, row0, head0 * p.q_at.head, b * p.q_at.batch);
+            load_k(0);
+            load_v(0);
+        }
     }
-    if (BIAS) load_bias(bias, p.h, head0, threadIdx.x, kFwdThreads);
+    if constexpr (BIAS) {
+        load_runs(bias, p.h, warp, kFwdThreads / 32, lane);
+        for (int r = threadIdx.x; r < p.h.n_runs; r += kFwdThreads) bias.value[r] = heads_run_bias(p.h, r, head0);
+    }
     if (warp == 1) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), kTmemCols);
         ptx::tmem_relinquish();
@@ -139,24 +161,12 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 
     if (warp == 0) {
         // ---- TMA producer ------------------------------------------------------------------------------
-        if (lane == 0 && kv_tiles > 0) {
-            ptx::mbar_arrive_expect_tx(q_full, box_rows * D * 2);
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c)
-                ptx::tma_load_4d(q_smem + c * (kTile * 128), &map_q, q_full, c * 64, row0, head0 * p.q_at.head, b * p.q_at.batch);
-            for (int j = 0; j < kv_tiles; ++j) {
-                const uint32_t ph = j & 1;
-                const int key0 = (tile_first + j) * kTile;
-                if (!bounded_wait(wctx, k_empty, ph ^ 1, 0x04010000u | (j & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(k_full, S::kOperand);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    ptx::tma_load_4d(k_smem + c * (kTile * 128), &map_k, k_full, c * 64, key0, hk * p.k_at.head, b * p.k_at.batch);
-                if (!bounded_wait(wctx, v_empty, ph ^ 1, 0x04020000u | (j & 0xffff))) break;
-                ptx::mbar_arrive_expect_tx(v_full, S::kOperand);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, v_full, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
+        if (lane == 0) {
+            for (int j = 1; j < kv_tiles; ++j) {
+                if (!bounded_wait(wctx, k_empty, (j & 1) ^ 1, 0x04010000u | (j & 0xffff))) break;
+                load_k(j);
+                if (!bounded_wait(wctx, v_empty, (j & 1) ^ 1, 0x04020000u | (j & 0xffff))) break;
+                load_v(j);
             }
         }
         __syncwarp();
@@ -207,8 +217,7 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         float m_run = -CUDART_INF_F;      // the max the exponentials are taken against (log2 units)
         float l_run = 0.0f;               // running sum over this thread's columns
         bool ok = true;
-        WarpBias wb;
-        wb.reset();
+        WarpBias wb(p.h);
         for (int j = 0; j < kv_tiles && ok; ++j) {
             const int key0 = (tile_first + j) * kTile + half * (kTile / 2);
             float c = p.h.scale_log2, add = 0.0f;               // a score in log2 units is c * s + add

@@ -90,31 +90,56 @@ __device__ __forceinline__ bool warp_spin(const WaitCtx& ctx, uint32_t bar, uint
 
 // ---- the bias --------------------------------------------------------------------------------------------------------
 // A warp works on 32 x 64 blocks of scores, which span 95 distances. Where they all fall into one run (far from the
-// diagonal: every distance beyond max_distance) the bias is one number; else the warp looks the 95 up (a binary search
-// each, three a lane) into its own stretch of shared memory. The range of the run is kept, so that neighbouring
-// blocks of a far stretch cost two comparisons.
+// diagonal: every distance beyond max_distance) the bias is one number; else the warp copies the 95 values into its own
+// stretch of shared memory. The run of a distance comes from a table over the distances between the first run's last and the last
+// run's first, filled once per CTA, run by run (a binary search for every block took 1900 cycles of the 4000 a block cost);
+// schemes that spread over more than kNear distances are searched. The range of the last single run is kept, so that neighbouring blocks of a
+// far stretch cost two comparisons.
+constexpr int kNear = 4096;
 struct BiasShared {
     int first[kHeadsMaxRuns];
     float value[kHeadsMaxRuns];         // of the head, log2 units
     float by_dist[8][96];               // one row per warp
+    uint8_t near_run[kNear];            // run of distance near_first + i
 };
 static_assert(offsetof(BiasShared, by_dist) % 16 == 0, "read as float4");
-// dq: sums along the diagonals of a warp's block of dS
-struct DiagShared {
-    float complete[8][64];              // what lane 31 saw: by column
-    float rest[8][4][32];               // what the lanes were left with after columns 15, 31, 47, 63
+// The distances near_run covers: from the last one of run 0 to the first one of the last run.
+struct NearRuns {
+    int first, count;                   // count 0: not used
+    __device__ __forceinline__ NearRuns(const HeadsParams& p) {
+        first = p.n_runs > 1 ? p.run_first[1] - 1 : 0;
+        const int span = p.n_runs > 1 ? p.run_first[p.n_runs - 1] - first + 1 : 1;
+        count = span <= kNear ? span : 0;
+    }
 };
+// The part of the shared tables that does not depend on the head; `warp` of `warps`.
+__device__ __forceinline__ void load_runs(BiasShared& s, const HeadsParams& p, int warp, int warps, int lane) {
+    const NearRuns near(p);
+    for (int r = warp; r < p.n_runs; r += warps) {
+        if (lane == 0) s.first[r] = p.run_first[r];
+        if (near.count) {
+            const int from = r == 0 ? 0 : p.run_first[r] - near.first, to = r + 1 == p.n_runs ? near.count : p.run_first[r + 1] - near.first;
+            for (int i = from + lane; i < to; i += 32) s.near_run[i] = (uint8_t)r;
+        }
+    }
+}
 struct WarpBias {
     int lo, hi;                         // distances [lo, hi) have the bias `same`
     int run;                            // its run
     float same;
+    NearRuns near;
+    __device__ __forceinline__ WarpBias(const HeadsParams& p) : near(p) { reset(); }
     __device__ __forceinline__ void reset() { lo = 0; hi = 0; run = 0; same = 0.0f; }
+    __device__ __forceinline__ int run_of(const BiasShared& s, int n_runs, int dist) const {
+        if (near.count) return s.near_run[min(max(dist - near.first, 0), near.count - 1)];
+        return heads_run_of(s.first, n_runs, dist);
+    }
     // Distances d0 .. d0 + 94. True: all in one run. False: s.by_dist[warp][0 .. 94] holds their biases. `value`: by run.
     __device__ __forceinline__ bool block(BiasShared& s, const float* value, int warp, int lane, int n_runs, int d0) {
         if (d0 >= lo && d0 + 94 < hi) return true;
         int r[3];
 #pragma unroll
-        for (int k = 0; k < 3; ++k) r[k] = heads_run_of(s.first, n_runs, d0 + 32 * k + lane);
+        for (int k = 0; k < 3; ++k) r[k] = run_of(s, n_runs, d0 + 32 * k + lane);
         const int ra = __shfl_sync(0xffffffffu, r[0], 0), rb = __shfl_sync(0xffffffffu, r[2], 30);
         if (ra == rb) {
             lo = ra == 0 ? INT_MIN : s.first[ra];
@@ -130,13 +155,12 @@ struct WarpBias {
         return false;
     }
 };
-__device__ __forceinline__ void load_bias(BiasShared& s, const HeadsParams& p, int head, int tid, int threads) {
-    for (int r = tid; r < p.n_runs; r += threads) {
-        s.first[r] = p.run_first[r];
-        s.value[r] = heads_run_bias(p, r, head);
-    }
-}
 
+// dq: sums along the diagonals of a warp's block of dS
+struct DiagShared {
+    float complete[8][64];              // what lane 31 saw: by column
+    float rest[8][4][32];               // what the lanes were left with after columns 15, 31, 47, 63
+};
 // ---- the order of the work items -----------------------------------------------------------------------------------------------
 // Causal tiles differ in length. Dealt longest first over many units the SMs finish together; dealt unit by unit the last units'
 // longest tiles run alone (16 units of 2048 keys on 148 SMs: 184 us against 118). But CTAs that run at the same time should share
