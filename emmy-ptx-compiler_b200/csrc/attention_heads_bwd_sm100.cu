@@ -59,15 +59,12 @@ struct BwdSmem {
     static constexpr int kBarOffset = kRowsOffset + kStages * 512;
     static constexpr int kBiasOffset = kBarOffset + 512;
     static constexpr int kSumsOffset = kBiasOffset + (int)sizeof(BiasShared);
-    static constexpr int kDiagOffset = kSumsOffset + 8 * kHeadsMaxRuns * 4;
-    static constexpr int kTotal = kDiagOffset + (int)sizeof(DiagShared) + 1024;
+    static constexpr int kTotal = kSumsOffset + 8 * kHeadsMaxRuns * 4 + 1024;
 };
 
-// The power of two dS is scaled by in f16: |dS| 2^14 g <= 2^15 from |dO . v - D| <= 2 max|dO| max|v|. 1 in bf16.
-template <bool BF16>
-__device__ __forceinline__ float ds_scale(const HeadsGrads& g, int64_t bk, int64_t all) {
-    if constexpr (BF16) return 1.0f;
-    const float bound = sqrtf(g.amax[bk]) * sqrtf(g.amax[all + bk]);
+// The power of two dS is scaled by in f16: |dS| 2^14 g <= 2^15 from |dO . v - D| <= 2 max|dO| max|v|, given the largest squared row norms.
+__device__ __forceinline__ float ds_scale(float do_norm, float v_norm) {
+    const float bound = sqrtf(do_norm) * sqrtf(v_norm);
     if (!(bound > 0.0f) || !(bound < CUDART_INF_F)) return 1.0f;
     return __int_as_float(((int)fminf(fmaxf(floorf(-log2f(bound)), -100.0f), 100.0f) + 127) << 23);
 }
@@ -200,14 +197,18 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
     const int x = (warp - 2) >> 2;                              // group of the warps 2 to 9
     const int key = key0 + (warp & 3) * 32 + lane;
+    // loads from here to the barrier are in flight together
     uint4 a_row[D / 8];
-    float g_scale = 1.0f;
+    float do_norm = 0.0f, v_norm = 0.0f;
     if (warp >= 2 && n_it > 0) {
         if constexpr (kKvInTmem)                                // group 0 brings K to tensor memory, group 1 V
             load_row<D / 2>(a_row, x ? static_cast<const uint16_t*>(p.g.v) + b * p.h.v_s[0] + hk * p.h.v_s[1] + key * p.h.v_s[2]
                                      : static_cast<const uint16_t*>(p.g.k) + b * p.h.k_s[0] + hk * p.h.k_s[1] + key * p.h.k_s[2],
                             key < n_keys);
-        g_scale = ds_scale<BF16>(p.g, bk, (int64_t)p.h.batch * p.h.kv_heads);
+        if (!BF16) {
+            do_norm = __ldg(p.g.amax + bk);
+            v_norm = __ldg(p.g.amax + (int64_t)p.h.batch * p.h.kv_heads + bk);
+        }
     }
     if constexpr (BIAS) load_runs(bias, p.h, warp, kBwdThreads / 32, lane);
     if (warp == 1) {
@@ -282,6 +283,7 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(kv_ready);
         }
+        const float g_scale = BF16 ? 1.0f : ds_scale(do_norm, v_norm);
         const float2 g2 = make_float2(g_scale, g_scale);
         bool ok = true;
         WarpBias wb(p.h);
@@ -442,8 +444,8 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 // to the warp's sum of that run when the run changes; other blocks are added up along their 95 diagonals, without atomics: a partial
 // sum moves one lane up per column, so that it follows its diagonal and is complete when it reaches lane 31. Four chains of 16 columns run side by
 // side (one of 64 was bound by the shuffle's latency: 55 us of dq for 96 units of 512 x 512 x 64, 8 tiles each); what the lanes hold
-// after a chain's last column are partial sums of the 32 diagonals that go on into the next. Each run the block touches is then
-// added up by one lane, whole groups of eight diagonals at a time.
+// after a chain's last column are partial sums of the 32 diagonals that go on into the next. A scan over the diagonals that stops
+// where a run begins then gives each run's sum to its last diagonal's lane.
 struct RunSums {
     float acc;              // this thread's part of the run
     int run;
@@ -474,7 +476,6 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 96);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
-    DiagShared& diag = *reinterpret_cast<DiagShared*>(smem_gen + S::kDiagOffset);
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const WorkItem work = work_item(blockIdx.x, p.h.batch * p.h.heads, p.q_tiles, p.chunk_dq);
@@ -508,8 +509,10 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
     const int x = (warp - 2) >> 2;                              // group of the warps 2 to 9
     const int row = row0 + (warp & 3) * 32 + lane;
+    // loads from here to the barrier are in flight together
     uint4 a_row[D / 8];
-    float nlse = 0.0f, ndelta = 0.0f, g_scale = 1.0f;
+    float nlse = 0.0f, ndelta = 0.0f, do_norm = 0.0f, v_norm = 0.0f, run_bias = 0.0f;
+    if (BIAS && (int)threadIdx.x < p.h.n_runs) run_bias = heads_run_bias(p.h, threadIdx.x, h);
     if (warp >= 2) {                                            // group 0 brings Q to tensor memory, group 1 dO
         load_row<D / 2>(a_row, x ? static_cast<const uint16_t*>(p.g.d_o) + b * p.h.do_s[0] + h * p.h.do_s[1] + row * p.h.do_s[2]
                                  : static_cast<const uint16_t*>(p.g.q) + b * p.h.q_s[0] + h * p.h.q_s[1] + row * p.h.q_s[2],
@@ -517,11 +520,14 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         const int64_t at_row = (int64_t)bh * p.g.pad_q + row;
         nlse = p.g.lse2[at_row];
         ndelta = p.g.delta[at_row];
-        g_scale = ds_scale<BF16>(p.g, b * p.h.kv_heads + hk, (int64_t)p.h.batch * p.h.kv_heads);
+        if (!BF16) {
+            do_norm = __ldg(p.g.amax + b * p.h.kv_heads + hk);
+            v_norm = __ldg(p.g.amax + (int64_t)p.h.batch * p.h.kv_heads + b * p.h.kv_heads + hk);
+        }
     }
     if constexpr (BIAS) {
         load_runs(bias, p.h, warp, kBwdThreads / 32, lane);
-        for (int r = threadIdx.x; r < p.h.n_runs; r += kBwdThreads) bias.value[r] = heads_run_bias(p.h, r, h);
+        if ((int)threadIdx.x < p.h.n_runs) bias.value[threadIdx.x] = run_bias;
     }
     if (warp == 1) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
@@ -598,6 +604,7 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(a_ready);
         }
+        const float g_scale = BF16 ? 1.0f : ds_scale(do_norm, v_norm);
         const float2 nd2 = make_float2(ndelta, ndelta), g2 = make_float2(g_scale, g_scale);
         const int sees = p.h.causal ? min(n_keys, row + offset + 1) : n_keys;
         const bool want_bias = BIAS && p.g.dtable != nullptr;
@@ -696,45 +703,41 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                                 const float below = __shfl_up_sync(0xffffffffu, __uint_as_float(r[chain + i - 1]), 1);
                                 r[chain + i] = __float_as_uint(fmaf(below, go_on, __uint_as_float(r[chain + i])));
                             }
+                        float* by_diag = bias.by_dist[w];                   // the biases have been read
                         if (lane == 31) {
 #pragma unroll
-                            for (int i = 0; i < 64; i += 4) *reinterpret_cast<uint4*>(&diag.complete[w][i]) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+                            for (int i = 0; i < 64; i += 4) *reinterpret_cast<uint4*>(by_diag + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
                         }
-#pragma unroll
-                        for (int chain = 0; chain < 4; ++chain) diag.rest[w][chain][lane] = lane == 31 ? 0.0f : __uint_as_float(r[16 * chain + 15]);
                         __syncwarp();
-                        // lane: diagonals 3 lane .. 3 lane + 2; lane l's rest of chain c belongs to diagonal 16 c + 46 - l
-                        float d3[3];
+                        // lane l takes diagonals l, 32 + l, 64 + l; what lane k was left with by chain c belongs to diagonal 16 c + 46 - k
+                        // (lane 31's is complete)
+                        auto rest = [&](int chain, int t) {
+                            const int from = 16 * chain + 46 - t;
+                            const float v = __shfl_sync(0xffffffffu, __uint_as_float(r[16 * chain + 15]), from & 31);
+                            return from >= 0 && from < 31 ? v : 0.0f;
+                        };
+                        float d3[3] = {by_diag[lane] + rest(0, lane),
+                                       by_diag[32 + lane] + ((rest(0, 32 + lane) + rest(1, 32 + lane)) + rest(2, 32 + lane)),
+                                       rest(2, 64 + lane) + rest(3, 64 + lane)};
+                        // each run's sum by a scan that stops at the run's first diagonal, 32 diagonals at a time
+                        int run[3], start[3];
 #pragma unroll
                         for (int k = 0; k < 3; ++k) {
-                            const int t = 3 * lane + k;
-                            d3[k] = t < 64 ? diag.complete[w][t] : 0.0f;
+                            run[k] = wb.run_of(bias, p.h.n_runs, d0 + 32 * k + lane);
+                            start[k] = run[k] == 0 ? 0 : max(0, bias.first[run[k]] - d0 - 32 * k);
+                        }
 #pragma unroll
-                            for (int chain = 0; chain < 4; ++chain) {
-                                const int from = 16 * chain + 46 - t;
-                                if (from >= 0 && from < 32) d3[k] += diag.rest[w][chain][from];
+                        for (int off = 1; off < 32; off <<= 1)
+#pragma unroll
+                            for (int k = 0; k < 3; ++k) {
+                                const float v = __shfl_up_sync(0xffffffffu, d3[k], off);
+                                if (lane - off >= start[k]) d3[k] += v;
                             }
-                        }
-                        float* by_diag = bias.by_dist[w];                   // the biases have been read
 #pragma unroll
-                        for (int k = 0; k < 3; ++k) by_diag[3 * lane + k] = d3[k];
-                        __syncwarp();
-                        float* eights = diag.rest[w][0];                    // sums of eight neighbours
-                        if (lane < 12) {
-                            const float4 lo = *reinterpret_cast<const float4*>(by_diag + 8 * lane), hi = *reinterpret_cast<const float4*>(by_diag + 8 * lane + 4);
-                            eights[lane] = ((lo.x + lo.y) + (lo.z + lo.w)) + ((hi.x + hi.y) + (hi.z + hi.w));
-                        }
-                        __syncwarp();
-                        // runs the block touches, one lane each
-                        const int ra = wb.run_of(bias, p.h.n_runs, d0), rb = wb.run_of(bias, p.h.n_runs, d0 + 94);
-                        for (int run = ra + lane; run <= rb; run += 32) {
-                            int t = run == ra ? 0 : bias.first[run] - d0;
-                            const int to = run == rb ? 95 : bias.first[run + 1] - d0;
-                            float v = 0.0f;
-                            for (; t < to && (t & 7) != 0; ++t) v += by_diag[t];
-                            for (; t + 8 <= to; t += 8) v += eights[t >> 3];
-                            for (; t < to; ++t) v += by_diag[t];
-                            sums[run] += v;
+                        for (int k = 0; k < 3; ++k) {
+                            const int next = __shfl_down_sync(0xffffffffu, run[k], 1);
+                            if (lane == 31 || next != run[k]) sums[run[k]] += d3[k];
+                            __syncwarp();
                         }
                         __syncwarp();
                     } else {

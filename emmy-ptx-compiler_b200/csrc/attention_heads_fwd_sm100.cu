@@ -147,8 +147,10 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
     }
     if constexpr (BIAS) {
+        float run_bias = 0.0f;
+        if ((int)threadIdx.x < p.h.n_runs) run_bias = heads_run_bias(p.h, threadIdx.x, head0);
         load_runs(bias, p.h, warp, kFwdThreads / 32, lane);
-        for (int r = threadIdx.x; r < p.h.n_runs; r += kFwdThreads) bias.value[r] = heads_run_bias(p.h, r, head0);
+        if ((int)threadIdx.x < p.h.n_runs) bias.value[threadIdx.x] = run_bias;
     }
     if (warp == 1) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), kTmemCols);

@@ -117,7 +117,7 @@ __device__ __forceinline__ void load_runs(BiasShared& s, const HeadsParams& p, i
     const NearRuns near(p);
     for (int r = warp; r < p.n_runs; r += warps) {
         if (lane == 0) s.first[r] = p.run_first[r];
-        if (near.count) {
+        if (near.count) {                   // fills the runs the warp takes, 32 distances at a time
             const int from = r == 0 ? 0 : p.run_first[r] - near.first, to = r + 1 == p.n_runs ? near.count : p.run_first[r + 1] - near.first;
             for (int i = from + lane; i < to; i += 32) s.near_run[i] = (uint8_t)r;
         }
@@ -156,11 +156,6 @@ struct WarpBias {
     }
 };
 
-// dq: sums along the diagonals of a warp's block of dS
-struct DiagShared {
-    float complete[8][64];              // what lane 31 saw: by column
-    float rest[8][4][32];               // what the lanes were left with after columns 15, 31, 47, 63
-};
 // ---- the order of the work items -----------------------------------------------------------------------------------------------
 // Causal tiles differ in length. Dealt longest first over many units the SMs finish together; dealt unit by unit the last units'
 // longest tiles run alone (16 units of 2048 keys on 148 SMs: 184 us against 118). But CTAs that run at the same time should share
