@@ -1,13 +1,13 @@
 // Attention over heads, backward, on the tensor cores: f16 / bf16, d = 64 or 128.
 //
 // With P_ij = exp(s_ij - lse_i) and dS_ij = P_ij (dO_i . v_j - D_i), D_i = dO_i . O_i, the gradients are five products per tile of
-// queries x keys. Two kernels recompute P, each writing what its CTAs own, so nothing is accumulated across CTAs and results
+// queries x keys. Two kinds of CTAs recompute P, each writing what it owns, so nothing is accumulated across CTAs and results
 // are the same every time; the two score-sized products are done in both, seven in all where one kernel with atomic
 // additions into dQ would do five:
 //
-//   heads_dkv_kernel   a CTA owns 128 keys of a key head and walks the queries of every query head that reads it, 64 at a
-//                      time. Everything is transposed, keys are rows: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q.
-//   heads_dq_kernel    a CTA owns 128 queries and walks the keys, 64 at a time: S = Q K^T, dP = dO V^T, dQ += dS K.
+//   dkv_block   owns 128 keys of a key head and walks the queries of every query head that reads it, 64 at a time.
+//               Everything is transposed, keys are rows: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q.
+//   dq_block    owns 128 queries and walks the keys, 64 at a time: S = Q K^T, dP = dO V^T, dQ += dS K.
 //
 // One CTA per SM, 320 threads: warp 0 TMA (rings of 64-row stages), warp 1 issues the products, and two groups of four warps
 // do the arithmetic between them, taking the 64-column tiles in turn, one thread per row: while one group takes exponentials the products of
@@ -21,9 +21,8 @@
 //   columns, dkv: S 2 x 64, dP 2 x 64, dV d, dK d (K 32, V 32)      dq: S 2 x 64, dP 2 x 64, Q d / 2, dO d / 2, dQ d
 //
 // Row terms come from the rows kernel already negated and shifted: nlse2 = -lse log2(e) + shift, -inf for rows that see
-// nothing or lie behind seq_q, so that P = 2^(scale log2(e) q.k + bias + nlse2) needs no test. The shift scales P by what the
-// rounding to 16 bits wants: 1 + delta before bf16 values are cut (kCutScale), 2^14 for f16, whose small probabilities would
-// lose bits. dS inherits the factor and, in f16, a power of two per key head on top, chosen from the largest row norms of dO and V so that
+// nothing or lie behind seq_q, so that P = 2^(scale log2(e) q.k + bias + nlse2) needs no test. The shift scales P by what
+// 16 bits want: kCutScale before bf16 values are cut, 2^14 for f16, whose small probabilities would lose bits. dS inherits the factor and, in f16, a power of two per key head on top, chosen from the largest row norms of dO and V so that
 // |dS| stays below 2^15: a tiny or huge incoming gradient keeps its bits. All factors but the cut's are exact and taken out at the end.
 #include <math_constants.h>
 
@@ -38,11 +37,16 @@ constexpr int kF16Shift = 14;
 struct BwdParams {
     HeadsParams h;
     HeadsGrads g;
-    MapAt q_at, k_at, v_at, do_at;
+    MapAt q_at, k_at, v_at, do_at, dq_at, dk_at, dv_at;
     int q_tiles, k_tiles;
     int chunk_dkv, chunk_dq;            // of units, see work_item
+    int dkv_blocks;                     // blocks from here on work on dQ
     unsigned long long wait_limit_ns;
     uint32_t* status;
+};
+struct BwdMaps {
+    CUtensorMap q, d_o, k, v;           // stages of 64 rows
+    CUtensorMap k_tile, v_tile, dq, dk, dv;     // 128 rows
 };
 
 __device__ uint32_t g_bwd_status;
@@ -120,9 +124,8 @@ struct Products {
     }
 };
 template <int D, bool BF16, bool BIAS>
-__global__ void __launch_bounds__(kBwdThreads, 1)
-heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                 const __grid_constant__ CUtensorMap map_do, const __grid_constant__ BwdParams p) {
+__device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, int item) {
+    const CUtensorMap &map_q = m.q, &map_k = m.k_tile, &map_v = m.v_tile, &map_do = m.d_o, &map_dk = m.dk, &map_dv = m.dv;
     using S = BwdSmem<D>;
     using Mma = Products<D, BF16>;
     constexpr int kChunks = D / 64, kStages = S::kStages;
@@ -137,13 +140,13 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const uint32_t rows_smem = smem_base + S::kRowsOffset;
     const uint32_t bar_base = smem_base + S::kBarOffset;
     const uint32_t kv_ready = bar_base, acc_full = bar_base + 16, s_full = bar_base + 24 /* per group */, dp_full = bar_base + 40,
-                   p_ready = bar_base + 56, ds_ready = bar_base + 72, full = bar_base + 128, empty = full + 8 * kStages;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 96);
+                   p_ready = bar_base + 56, ds_ready = bar_base + 72, staged = bar_base + 104, full = bar_base + 128, empty = full + 8 * kStages;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 120);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const WorkItem work = work_item(blockIdx.x, p.h.batch * p.h.kv_heads, p.k_tiles, p.chunk_dkv);
+    const WorkItem work = work_item(item, p.h.batch * p.h.kv_heads, p.k_tiles, p.chunk_dkv);
     const int kt = work.tile, bk = work.unit;                   // causal: the first key tiles see the most queries
     const int b = bk / p.h.kv_heads, hk = bk % p.h.kv_heads;
     const int key0 = kt * kTile;
@@ -176,7 +179,7 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (threadIdx.x == 0) {
         ptx::mbar_init(kv_ready, kKvInTmem ? 8 : 1); ptx::mbar_init(acc_full, 1);
         for (int x = 0; x < 2; ++x) {
-            ptx::mbar_init(s_full + 8 * x, 1); ptx::mbar_init(dp_full + 8 * x, 1); ptx::mbar_init(p_ready + 8 * x, 4); ptx::mbar_init(ds_ready + 8 * x, 4);
+            ptx::mbar_init(s_full + 8 * x, 1); ptx::mbar_init(dp_full + 8 * x, 1); ptx::mbar_init(p_ready + 8 * x, 4); ptx::mbar_init(ds_ready + 8 * x, 4); ptx::mbar_init(staged + 8 * x, 4);
         }
         for (int s = 0; s < kStages; ++s) {
             ptx::mbar_init(full + 8 * s, 1); ptx::mbar_init(empty + 8 * s, 1);
@@ -192,7 +195,8 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, kv_ready, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
                 }
             }
-            for (; load_it < n_it && load_it < kStages; advance()) load_stage(load_s, load_gi, load_qt);
+            load_stage(load_s, load_gi, load_qt);
+            advance();
         }
     }
     const int x = (warp - 2) >> 2;                              // group of the warps 2 to 9
@@ -210,7 +214,7 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             v_norm = __ldg(p.g.amax + (int64_t)p.h.batch * p.h.kv_heads + bk);
         }
     }
-    if constexpr (BIAS) load_runs(bias, p.h, warp, kBwdThreads / 32, lane);
+    if constexpr (BIAS) load_runs(bias, p.h);
     if (warp == 1) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
         ptx::tmem_relinquish();
@@ -373,16 +377,15 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
                 for (int i = ch * 16; i < ch * 16 + 16; i += 2) {
                     const float4 nd = ndelta[i / 2];
-                    float2 e0 = e[i], e1 = e[i + 1];
-                    if constexpr (!BF16) { e0 = mul2(e0, g2); e1 = mul2(e1, g2); }
-                    float2 d0 = mul2(e0, add2(f2(r[2 * i], r[2 * i + 1]), make_float2(nd.x, nd.y)));
-                    float2 d1 = mul2(e1, add2(f2(r[2 * i + 2], r[2 * i + 3]), make_float2(nd.z, nd.w)));
+                    float2 d0 = mul2(e[i], add2(f2(r[2 * i], r[2 * i + 1]), make_float2(nd.x, nd.y)));
+                    float2 d1 = mul2(e[i + 1], add2(f2(r[2 * i + 2], r[2 * i + 3]), make_float2(nd.z, nd.w)));
                     if (masked) {                                       // dP may hold anything there
                         if (2 * i < hidden) d0.x = 0.0f;
                         if (2 * i + 1 < hidden) d0.y = 0.0f;
                         if (2 * i + 2 < hidden) d1.x = 0.0f;
                         if (2 * i + 3 < hidden) d1.y = 0.0f;
                     }
+                    if constexpr (!BF16) { d0 = mul2(d0, g2); d1 = mul2(d1, g2); }
                     pk[i - ch * 16] = operand_pair<BF16>(d0);
                     pk[i - ch * 16 + 1] = operand_pair<BF16>(d1);
                 }
@@ -403,11 +406,10 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (ok) {                                               // group 0 writes dV, group 1 dK
             ptx::tc_fence_after_sync();
             const float f = (BF16 ? 1.0f : 1.0f / (1 << kF16Shift)) * (x ? p.h.scale / g_scale : 1.0f);
-            uint16_t* out = x ? static_cast<uint16_t*>(p.g.dk) + b * p.h.dk_s[0] + hk * p.h.dk_s[1] + key * p.h.dk_s[2]
-                              : static_cast<uint16_t*>(p.g.dv) + b * p.h.dv_s[0] + hk * p.h.dv_s[1] + key * p.h.dv_s[2];
+            const uint32_t tile = smem_base + x * (2 * S::kStage);      // every load has been used: the tile is staged where the operands were
 #pragma unroll 1
             for (int col = 0; col < D; col += 32) {
-                uint32_t r[32];
+                uint32_t r[32], v[16];
                 if (n_it > 0) {
                     ptx::tmem_ld_32x32b_x32(tmem_base + lane_base + (x ? kColDK : kColDV) + col, r);
                     ptx::tmem_ld_wait();
@@ -415,16 +417,20 @@ heads_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
                     for (int i = 0; i < 32; ++i) r[i] = 0;
                 }
-                if (key < p.h.seq_k) {
-                    uint4* dst = reinterpret_cast<uint4*>(out + col);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t v[4];
+                for (int i = 0; i < 16; ++i) v[i] = round_pair<BF16>(__uint_as_float(r[2 * i]) * f, __uint_as_float(r[2 * i + 1]) * f);
+                stage_row(tile, quarter * 32 + lane, col, v);
+            }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(staged + 8 * x);
+            if (quarter == 2 && lane == 0 && bounded_wait(wctx, staged + 8 * x, 0, 0x050e0000u)) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = round_pair<BF16>(__uint_as_float(r[8 * q + 2 * i]) * f, __uint_as_float(r[8 * q + 2 * i + 1]) * f);
-                        dst[q] = make_uint4(v[0], v[1], v[2], v[3]);
-                    }
-                }
+                for (int c = 0; c < kChunks; ++c)               // rows behind seq_k are dropped
+                    ptx::tma_store_4d(x ? &map_dk : &map_dv, tile + c * (kTile * 128), c * 64, key0, hk * (x ? p.dk_at.head : p.dv_at.head),
+                                      b * (x ? p.dk_at.batch : p.dv_at.batch));
+                ptx::tma_store_commit();
+                ptx::tma_store_wait<0>();
             }
         }
     }
@@ -459,8 +465,8 @@ struct RunSums {
 };
 
 template <int D, bool BF16, bool BIAS>
-__global__ void __launch_bounds__(kBwdThreads, 1)
-heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ BwdParams p) {
+__device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, int item) {
+    const CUtensorMap &map_k = m.k, &map_v = m.v, &map_dq = m.dq;
     using S = BwdSmem<D>;
     using Mma = Products<D, BF16>;
     constexpr int kChunks = D / 64, kStages = S::kStagesDq;
@@ -471,14 +477,14 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     auto k_smem = [&](int s) { return smem_base + s * S::kStage; };
     auto v_smem = [&](int s) { return smem_base + (kStages + s) * S::kStage; };
     const uint32_t bar_base = smem_base + S::kBarOffset;
-    const uint32_t a_ready = bar_base, acc_full = bar_base + 8, s_full = bar_base + 16 /* per group */, dp_full = bar_base + 32, ds_ready = bar_base + 48, s_free = bar_base + 64,
+    const uint32_t a_ready = bar_base, acc_full = bar_base + 8, s_full = bar_base + 16 /* per group */, dp_full = bar_base + 32, ds_ready = bar_base + 48, s_free = bar_base + 64, staged = bar_base + 80,
                    full = bar_base + 128, empty = full + 8 * kStages;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 96);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 120);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const WorkItem work = work_item(blockIdx.x, p.h.batch * p.h.heads, p.q_tiles, p.chunk_dq);
+    const WorkItem work = work_item(item, p.h.batch * p.h.heads, p.q_tiles, p.chunk_dq);
     const int bh = work.unit, qt = p.h.causal ? p.q_tiles - 1 - work.tile : work.tile;
     const int b = bh / p.h.heads, h = bh % p.h.heads, hk = h / p.h.group;
     const int row0 = qt * kTile;
@@ -496,7 +502,7 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
     };
     if (threadIdx.x == 0) {
-        ptx::mbar_init(a_ready, 8); ptx::mbar_init(acc_full, 1);
+        ptx::mbar_init(a_ready, 8); ptx::mbar_init(acc_full, 1); ptx::mbar_init(staged, 8);
         for (int x = 0; x < 2; ++x) {
             ptx::mbar_init(s_full + 8 * x, 1); ptx::mbar_init(dp_full + 8 * x, 1); ptx::mbar_init(ds_ready + 8 * x, 4); ptx::mbar_init(s_free + 8 * x, 4);
         }
@@ -505,7 +511,7 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
         *abort_flag = 0;
         ptx::mbar_fence_init();
-        for (int it = 0; it < n_it && it < kStages; ++it) load_stage(it, it);           // these loads fly while the CTA sets itself up
+        if (n_it > 0) load_stage(0, 0);                         // flies while the CTA sets itself up
     }
     const int x = (warp - 2) >> 2;                              // group of the warps 2 to 9
     const int row = row0 + (warp & 3) * 32 + lane;
@@ -526,7 +532,7 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
     }
     if constexpr (BIAS) {
-        load_runs(bias, p.h, warp, kBwdThreads / 32, lane);
+        load_runs(bias, p.h);
         if ((int)threadIdx.x < p.h.n_runs) bias.value[threadIdx.x] = run_bias;
     }
     if (warp == 1) {
@@ -541,9 +547,9 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     if (warp == 0) {
         // ---- TMA producer ------------------------------------------------------------------------------
         if (lane == 0) {
-            int s = 0;
-            uint32_t phase = 0;                                 // of the first release
-            for (int it = kStages; it < n_it; ++it) {
+            int s = 1;
+            uint32_t phase = 1;
+            for (int it = 1; it < n_it; ++it) {
                 if (!bounded_wait(wctx, empty + 8 * s, phase, 0x06010000u | (it & 0xffff))) break;
                 load_stage(s, it);
                 if (++s == kStages) { s = 0; phase ^= 1; }
@@ -673,14 +679,12 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 uint32_t pk[16];
 #pragma unroll
                 for (int i = ch * 16; i < ch * 16 + 16; ++i) {
-                    float2 ee = e[i];
-                    if constexpr (!BF16) ee = mul2(ee, g2);
-                    float2 ds = mul2(ee, add2(f2(r[2 * i], r[2 * i + 1]), nd2));
+                    float2 ds = mul2(e[i], add2(f2(r[2 * i], r[2 * i + 1]), nd2));
                     if (masked) {
                         if (2 * i >= valid) ds.x = 0.0f;
                         if (2 * i + 1 >= valid) ds.y = 0.0f;
                     }
-                    pk[i - ch * 16] = operand_pair<BF16>(ds);
+                    pk[i - ch * 16] = operand_pair<BF16>(BF16 ? ds : mul2(ds, g2));
                     if constexpr (BIAS) {
                         r[2 * i] = __float_as_uint(ds.x);
                         r[2 * i + 1] = __float_as_uint(ds.y);
@@ -762,10 +766,9 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             ptx::tc_fence_after_sync();
             const float out = BF16 ? 1.0f : 1.0f / ((1 << kF16Shift) * g_scale);
             const float f = p.h.scale * out;
-            uint16_t* dq = static_cast<uint16_t*>(p.g.dq) + b * p.h.dq_s[0] + h * p.h.dq_s[1] + row * p.h.dq_s[2] + x * (D / 2);
 #pragma unroll 1
-            for (int ch = 0; ch < D / 64; ++ch) {
-                uint32_t r[32];
+            for (int ch = 0; ch < D / 64; ++ch) {               // every load has been used: the tile is staged where the operands were
+                uint32_t r[32], v[16];
                 if (n_it > 0) {
                     ptx::tmem_ld_32x32b_x32(tmem_base + lane_base + kColDQ + x * (D / 2) + ch * 32, r);
                     ptx::tmem_ld_wait();
@@ -773,22 +776,26 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
                     for (int i = 0; i < 32; ++i) r[i] = 0;
                 }
-                if (row < p.h.seq_q) {
-                    uint4* dst = reinterpret_cast<uint4*>(dq + ch * 32);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t v[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = round_pair<BF16>(__uint_as_float(r[8 * q + 2 * i]) * f, __uint_as_float(r[8 * q + 2 * i + 1]) * f);
-                        dst[q] = make_uint4(v[0], v[1], v[2], v[3]);
-                    }
-                }
+                for (int i = 0; i < 16; ++i) v[i] = round_pair<BF16>(__uint_as_float(r[2 * i]) * f, __uint_as_float(r[2 * i + 1]) * f);
+                stage_row(smem_base, quarter * 32 + lane, x * (D / 2) + ch * 32, v);
             }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(staged);
+            if (w == 0 && lane == 0 && bounded_wait(wctx, staged, 0, 0x060b0000u)) {
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c)               // rows behind seq_q are dropped
+                    ptx::tma_store_4d(&map_dq, smem_base + c * (kTile * 128), c * 64, row0, h * p.dq_at.head, b * p.dq_at.batch);
+                ptx::tma_store_commit();
+                ptx::tma_store_wait<0>();
+            }
+            __syncwarp();
             if constexpr (BIAS) {
                 if (want_bias) {
                     rs.flush(sums, lane);
                     __syncwarp();
-                    const float back = BF16 ? 1.0f / kCutScale : out;
+                    const float back = BF16 ? 1.0f / kCutScale : 1.0f / (1 << kF16Shift);
                     for (int r = lane; r < p.h.n_runs; r += 32)
                         p.g.run_sums[((int64_t)bh * p.g.q_tiles + qt * 8 + w) * p.h.n_runs + r] = sums[r] * back;
                 }
@@ -807,31 +814,37 @@ heads_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
 }
 
+// Both in one launch: the dq blocks fill the SMs that the last dkv blocks leave idle.
+template <int D, bool BF16, bool BIAS>
+__global__ void __launch_bounds__(kBwdThreads, 1) heads_bwd_kernel(const __grid_constant__ BwdMaps m, const __grid_constant__ BwdParams p) {
+    if ((int)blockIdx.x < p.dkv_blocks) dkv_block<D, BF16, BIAS>(m, p, blockIdx.x);
+    else dq_block<D, BF16, BIAS>(m, p, blockIdx.x - p.dkv_blocks);
+}
+
 template <int D, bool BF16>
 static int launch_bwd(BwdParams& p, cudaStream_t s) {
     const HeadsParams& h = p.h;
-    CUtensorMap mq, mk, mv, mk_tile, mv_tile, mdo;
-    int rc = make_map(&mq, &p.q_at, p.g.q, h.batch, h.heads, h.seq_q, D, h.q_s, kHalf, 1);
-    if (rc == EMMYB200_OK) rc = make_map(&mk, &p.k_at, p.g.k, h.batch, h.kv_heads, h.seq_k, D, h.k_s, kHalf, 1);
-    if (rc == EMMYB200_OK) rc = make_map(&mv, &p.v_at, p.g.v, h.batch, h.kv_heads, h.seq_k, D, h.v_s, kHalf, 1);
-    if (rc == EMMYB200_OK) rc = make_map(&mk_tile, &p.k_at, p.g.k, h.batch, h.kv_heads, h.seq_k, D, h.k_s, kTile, 1);
-    if (rc == EMMYB200_OK) rc = make_map(&mv_tile, &p.v_at, p.g.v, h.batch, h.kv_heads, h.seq_k, D, h.v_s, kTile, 1);
-    if (rc == EMMYB200_OK) rc = make_map(&mdo, &p.do_at, p.g.d_o, h.batch, h.heads, h.seq_q, D, h.do_s, kHalf, 1);
+    BwdMaps m;
+    int rc = make_map(&m.q, &p.q_at, p.g.q, h.batch, h.heads, h.seq_q, D, h.q_s, kHalf, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&m.d_o, &p.do_at, p.g.d_o, h.batch, h.heads, h.seq_q, D, h.do_s, kHalf, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&m.k, &p.k_at, p.g.k, h.batch, h.kv_heads, h.seq_k, D, h.k_s, kHalf, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&m.v, &p.v_at, p.g.v, h.batch, h.kv_heads, h.seq_k, D, h.v_s, kHalf, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&m.k_tile, &p.k_at, p.g.k, h.batch, h.kv_heads, h.seq_k, D, h.k_s, kTile, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&m.v_tile, &p.v_at, p.g.v, h.batch, h.kv_heads, h.seq_k, D, h.v_s, kTile, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&m.dq, &p.dq_at, p.g.dq, h.batch, h.heads, h.seq_q, D, h.dq_s, kTile, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&m.dk, &p.dk_at, p.g.dk, h.batch, h.kv_heads, h.seq_k, D, h.dk_s, kTile, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&m.dv, &p.dv_at, p.g.dv, h.batch, h.kv_heads, h.seq_k, D, h.dv_s, kTile, 1);
     if (rc != EMMYB200_OK) return rc;
     EMMY_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p.status), g_bwd_status));
     const int64_t kv_ctas = (int64_t)h.batch * h.kv_heads * p.k_tiles, q_ctas = (int64_t)h.batch * h.heads * p.q_tiles;
-    if (kv_ctas >= (1ll << 31) || q_ctas >= (1ll << 31)) return fail(EMMYB200_ERR_SHAPE, "attention_heads_bwd: the tiles exceed the grid limit");
+    if (kv_ctas + q_ctas >= (1ll << 31)) return fail(EMMYB200_ERR_SHAPE, "attention_heads_bwd: the tiles exceed the grid limit");
+    p.dkv_blocks = (int)kv_ctas;
     p.chunk_dkv = chunk_units(h.causal != 0, (int64_t)h.batch * h.kv_heads, (int64_t)h.seq_q * D * 4 * h.group);
     p.chunk_dq = chunk_units(h.causal != 0, (int64_t)h.batch * h.heads, (int64_t)h.seq_k * D * 4 / h.group);
-    auto dkv = h.n_runs ? heads_dkv_kernel<D, BF16, true> : heads_dkv_kernel<D, BF16, false>;
-    auto dq = h.n_runs ? heads_dq_kernel<D, BF16, true> : heads_dq_kernel<D, BF16, false>;
-    EMMY_CUDA(cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<D>::kTotal));
-    EMMY_CUDA(cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<D>::kTotal));
-    dkv<<<(unsigned)kv_ctas, kBwdThreads, BwdSmem<D>::kTotal, s>>>(mq, mk_tile, mv_tile, mdo, p);
-    rc = launch_status("heads_dkv_kernel");
-    if (rc != EMMYB200_OK) return rc;
-    dq<<<(unsigned)q_ctas, kBwdThreads, BwdSmem<D>::kTotal, s>>>(mk, mv, p);
-    return launch_status("heads_dq_kernel");
+    auto kernel = h.n_runs ? heads_bwd_kernel<D, BF16, true> : heads_bwd_kernel<D, BF16, false>;
+    EMMY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<D>::kTotal));
+    kernel<<<(unsigned)(kv_ctas + q_ctas), kBwdThreads, BwdSmem<D>::kTotal, s>>>(m, p);
+    return launch_status("heads_bwd_kernel");
 }
 
 }  // namespace heads

@@ -149,7 +149,7 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if constexpr (BIAS) {
         float run_bias = 0.0f;
         if ((int)threadIdx.x < p.h.n_runs) run_bias = heads_run_bias(p.h, threadIdx.x, head0);
-        load_runs(bias, p.h, warp, kFwdThreads / 32, lane);
+        load_runs(bias, p.h);
         if ((int)threadIdx.x < p.h.n_runs) bias.value[threadIdx.x] = run_bias;
     }
     if (warp == 1) {
@@ -349,18 +349,11 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     uint32_t o[32];
                     ptx::tmem_ld_32x32b_x32(o_row + ch * 32, o);
                     ptx::tmem_ld_wait();
-                    const int col = half * (D / 2) + ch * 32;   // first of these 32 columns
-                    const uint32_t row_smem = q_smem + (col / 64) * (kTile * 128) + row_in_tile * 128;
+                    uint32_t w[16];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint32_t piece = (uint32_t)((col % 64) / 8 + q) ^ (uint32_t)(row_in_tile & 7);
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            w[i] = empty ? 0u : round_pair<BF16>(__uint_as_float(o[8 * q + 2 * i]) * inv, __uint_as_float(o[8 * q + 2 * i + 1]) * inv);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_smem + piece * 16), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                                     : "memory");
-                    }
+                    for (int i = 0; i < 16; ++i)
+                        w[i] = empty ? 0u : round_pair<BF16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+                    stage_row(q_smem, row_in_tile, half * (D / 2) + ch * 32, w);
                 }
                 ptx::fence_proxy_async_smem();
                 __syncwarp();

@@ -12,10 +12,10 @@ namespace emmy {
 namespace heads {
 
 constexpr int kTile = 128;              // query rows and keys of a tile
-// bf16 operands are made by cutting the fp32 pattern (one byte permute per pair; a conversion would run on the
-// transcendental unit next to the exponentials). The cut loses half a step, 2^-8 of a value with mantissa 1, on average 2^-8 / ln 4 of
+// bf16 operands of second products are cut from the fp32 pattern (one byte permute per pair): a conversion would run on the
+// transcendental unit next to the exponentials. A cut loses half a step, 2^-8 of a value with mantissa 1, on average 2^-8 / ln 4 of
 // values spread evenly in magnitude: they are scaled by 1 + 2^-8 / ln 4 first, which leaves no mean error and at most 1.28 times the
-// 2^-8 of a rounding.
+// 2^-8 of a rounding. f16 operands are converted: the same cut for f16 needs two more operations per value and was 5 % slower.
 constexpr float kCutScale = 1.0028178f;
 constexpr float kCutScaleLog2 = 0.0040594572f;      // its log2
 
@@ -49,7 +49,7 @@ __device__ __forceinline__ uint32_t round_pair(float lo, float hi) {
         return *reinterpret_cast<uint32_t*>(&v);
     }
 }
-// Operands of a second product: bf16 values already scaled by 1 + 2^-9 are cut, f16 ones rounded.
+// Operands of a second product: bf16 values already scaled by kCutScale are cut, f16 ones rounded.
 template <bool BF16>
 __device__ __forceinline__ uint32_t operand_pair(float2 v) {
     if constexpr (BF16) return __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
@@ -112,15 +112,16 @@ struct NearRuns {
         count = span <= kNear ? span : 0;
     }
 };
-// The part of the shared tables that does not depend on the head; `warp` of `warps`.
-__device__ __forceinline__ void load_runs(BiasShared& s, const HeadsParams& p, int warp, int warps, int lane) {
+// The part of the shared tables that does not depend on the head: thread r fills in run r.
+__device__ __forceinline__ void load_runs(BiasShared& s, const HeadsParams& p) {
+    const int r = threadIdx.x;
+    if (r >= p.n_runs) return;
     const NearRuns near(p);
-    for (int r = warp; r < p.n_runs; r += warps) {
-        if (lane == 0) s.first[r] = p.run_first[r];
-        if (near.count) {                   // fills the runs the warp takes, 32 distances at a time
-            const int from = r == 0 ? 0 : p.run_first[r] - near.first, to = r + 1 == p.n_runs ? near.count : p.run_first[r + 1] - near.first;
-            for (int i = from + lane; i < to; i += 32) s.near_run[i] = (uint8_t)r;
-        }
+    const int mine = p.run_first[r];
+    s.first[r] = mine;
+    if (near.count) {
+        const int to = r + 1 == p.n_runs ? near.count : p.run_first[r + 1] - near.first;
+        for (int i = r == 0 ? 0 : mine - near.first; i < to; ++i) s.near_run[i] = (uint8_t)r;
     }
 }
 struct WarpBias {
@@ -197,6 +198,18 @@ inline int make_map(CUtensorMap* map, MapAt* at, const void* base, int64_t batch
     const uint64_t stride[3] = {row_s, at->head ? (uint64_t)s[1] : row_s, at->batch ? (uint64_t)s[0] : row_s};
     const uint32_t box[4] = {64, (uint32_t)box_rows, (uint32_t)box_heads, 1};
     return make_tensor_map_4d(map, base, extent, stride, box);
+}
+
+// 32 columns of an output row (from `col` on, a multiple of 32) into a tile of 128 rows staged for a TMA store: pieces of 128 rows x
+// 64 columns, 128-byte swizzle. `w`: the 16-bit pairs.
+__device__ __forceinline__ void stage_row(uint32_t tile, int row, int col, const uint32_t (&w)[16]) {
+    const uint32_t at = tile + (col / 64) * (kTile * 128) + row * 128;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t piece = (uint32_t)((col % 64) / 8 + q) ^ (uint32_t)(row & 7);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + piece * 16), "r"(w[4 * q]), "r"(w[4 * q + 1]), "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
+                     : "memory");
+    }
 }
 
 }  // namespace heads
