@@ -231,7 +231,7 @@ static int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 static BwdLayout bwd_layout(const emmyb200_attention_heads_desc* c) {
     BwdLayout w;
     w.pad_q = (c->seq_q + 127) / 128 * 128;
-    w.parts = w.pad_q / 128 * 8;                // tensor cores: eight warps per 128 queries; CUDA cores: one part per 64
+    w.parts = w.pad_q / 128 * 8;                // tensor cores: eight warps per 128 queries; CUDA cores: one part per 16 or 64
     const int64_t rows = round256(c->batch * c->heads * w.pad_q * 4);
     w.delta_at = rows;
     w.sums_at = 2 * rows;
@@ -333,7 +333,8 @@ extern "C" int emmyb200_attention_heads_bwd(const emmyb200_attention_heads_desc*
     g.amax = reinterpret_cast<float*>(ws + w.amax_at);
     const bool tensor_cores = has_q && has_k && heads_bwd_sm100_takes(p, c->dtype, (int)c->d, g);
     const bool norms = tensor_cores && c->dtype == EMMYB200_F16;
-    g.q_tiles = (int)(tensor_cores ? w.parts : (c->seq_q + kCoresTile - 1) / kCoresTile);
+    const int cores_rows = 16 * heads_cores_rows(p);
+    g.q_tiles = (int)(tensor_cores ? w.parts : (c->seq_q + cores_rows - 1) / cores_rows);
     if (tensor_cores) {
         if (norms) EMMY_CUDA(cudaMemsetAsync(g.amax, 0, 2 * c->batch * c->kv_heads * 4, s));
         rc = norms ? launch_rows16<__half, true>(p, g, (int)c->d, heads_bwd_shift(c->dtype), s)

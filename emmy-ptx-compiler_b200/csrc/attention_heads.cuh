@@ -83,7 +83,8 @@ __device__ __forceinline__ int heads_run_of(const int* first, int n_runs, int di
 // CUDA cores, fp32 arithmetic: any dtype, d = 32, 64, 96 or 128, any alignment.
 int heads_fwd_cores(int dtype, int d, const HeadsParams& p, const void* Q, const void* K, const void* V, void* O, float* lse, cudaStream_t s);
 int heads_bwd_cores(int dtype, int d, const HeadsParams& p, const HeadsGrads& g, cudaStream_t s);
-constexpr int kCoresTile = 64;                  // query and key tile of the CUDA-core kernels
+constexpr int kCoresTile = 64;                  // rows the CUDA-core kernels stage at a time
+int heads_cores_rows(const HeadsParams& p);     // rows per thread; a block owns 16 times as many
 
 // Tensor cores: 16-bit operands with d = 64 or 128 that TMA can address (heads_sm100_takes).
 struct FwdPlan {

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libemmyb200.so"
@@ -630,105 +631,92 @@ def relative_runs(buckets: int, max_distance: int = 128, bidirectional: bool = T
     return [(first[i], bucket[i]) for i in range(n)]
 
 
+def _layout(t):
+    """What a call checks of a tensor: all that its plan depends on."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
 @functools.lru_cache(maxsize=512)
-def _heads_desc(backward: bool, dtype: int, flags: int, q_shape, k_shape, strides, scale: float, bias):
-    """The C description of a call and its workspace bytes, by sizes alone (`bias`: dtype, strides, buckets, max_distance, bidirectional)."""
+def _heads_plan(who: str, backward: bool, scale, causal: bool, align: str, max_distance: int, bidirectional: bool, key_lens, bias_table, lse, dtable,
+                workspace, q, k, v, o, do=None, dq=None, dk=None, dv=None):
+    """The checked C description of a call and its workspace bytes. Depends on layouts and settings alone: a program's
+    repeated calls find it here."""
+    import torch
+    (q_shape, _, dtype, device), k_shape = q, k[0]
+    if len(q_shape) != 4 or len(k_shape) != 4 or len(v[0]) != 4:
+        raise ValueError(f"{who}: q is [batch, heads, seq_q, d], k and v [batch, kv_heads, seq_k, d]")
+    if k_shape != v[0] or q_shape[0] != k_shape[0] or q_shape[3] != k_shape[3]:
+        raise ValueError(f"{who}: shapes do not agree: {tuple(q_shape)}, {tuple(k_shape)}, {tuple(v[0])}")
+    floats = (torch.float32, torch.float16, torch.bfloat16)
+    if dtype not in floats:
+        raise TypeError(f"{who}: float32, float16 or bfloat16")
+    for name, t, shape in (("q", q, q_shape), ("k", k, k_shape), ("v", v, k_shape), ("o", o, q_shape), ("do", do, q_shape), ("dq", dq, q_shape),
+                           ("dk", dk, k_shape), ("dv", dv, k_shape)):
+        if t is None:
+            continue
+        if t[3].type != "cuda":
+            raise RuntimeError("emmyb200 kernels take CUDA tensors only (there is no CPU path)")
+        if t[0] != shape or t[2] != dtype or t[3] != device:
+            raise ValueError(f"{who}: {name} is {tuple(t[0])} {t[2]} on {t[3]}; wanted {tuple(shape)} {dtype} on {device}")
+        if t[1][3] != 1:
+            raise ValueError(f"{who}: the head dim of {name} must be contiguous")
+
+    def dense(t):
+        return all(s == math.prod(t[0][i + 1:]) for i, s in enumerate(t[1]) if t[0][i] > 1) or 0 in t[0]
+    if key_lens is not None and (key_lens[2] != torch.int32 or key_lens[0] != q_shape[:1] or key_lens[3] != device or not dense(key_lens)):
+        raise ValueError(f"{who}: key_lens is a contiguous int32 vector [batch] on {device}")
+    if bias_table is not None and (len(bias_table[0]) != 2 or bias_table[0][1] != q_shape[1] or bias_table[3] != device or bias_table[2] not in floats):
+        raise ValueError(f"{who}: bias_table is a float [buckets, heads] tensor on {device}")
+    if lse[2] != torch.float32 or lse[0] != q_shape[:3] or lse[3] != device or not dense(lse):
+        raise ValueError(f"{who}: lse is a contiguous float32 [batch, heads, seq_q] tensor")
+    if dtable is not None and (bias_table is None or dtable[0] != bias_table[0] or dtable[2] != bias_table[2] or dtable[3] != device or not dense(dtable)):
+        raise ValueError(f"{who}: dtable is a contiguous tensor like bias_table")
+    if align not in ("start", "end"):
+        raise ValueError(f"{who}: align is 'start' or 'end'")
+    codes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
     desc = HeadsDesc()
-    desc.dtype, desc.flags, desc.scale = dtype, flags, scale
+    desc.dtype, desc.flags = codes[dtype], (HEADS_CAUSAL if causal else 0) | (HEADS_ALIGN_END if align == "end" else 0)
+    desc.scale = q_shape[3] ** -0.5 if scale is None else scale
     desc.batch, desc.heads, desc.seq_q, desc.d = q_shape
     desc.kv_heads, desc.seq_k = k_shape[1], k_shape[2]
-    for name, stride in zip(("q", "k", "v", "o", "do", "dq", "dk", "dv"), strides):
-        getattr(desc, f"{name}_stride")[:] = stride
-    if bias is not None:
-        desc.bias_dtype, desc.bias_stride[:], desc.buckets = bias[0], bias[1], bias[2]
-        desc.n_runs, desc.run_first, desc.run_bucket = _relative_runs(*bias[2:])
+    for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("do", do), ("dq", dq), ("dk", dk), ("dv", dv)):
+        if t is not None:
+            getattr(desc, f"{name}_stride")[:] = t[1][:3]
+    if bias_table is not None:
+        desc.bias_dtype, desc.bias_stride[:], desc.buckets = codes[bias_table[2]], bias_table[1], bias_table[0][0]
+        desc.n_runs, desc.run_first, desc.run_bucket = _relative_runs(bias_table[0][0], max_distance, bidirectional)
     need = library().emmyb200_attention_heads_workspace_bytes(ctypes.byref(desc), 1 if backward else 0)
     if need < 0:
         raise KernelError(-1, library().emmyb200_last_error().decode())
-    return desc, need
-
-
-def _heads_call(who: str, q, k, v, key_lens, bias_table, same_as_q: dict, same_as_k: dict):
-    """Checks what both directions share: shapes, one dtype and device, contiguous head dims."""
-    import torch
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
-        raise ValueError(f"{who}: q is [batch, heads, seq_q, d], k and v [batch, kv_heads, seq_k, d]")
-    if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"{who}: shapes do not agree: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-        raise TypeError(f"{who}: float32, float16 or bfloat16")
-    for name, t, shape in [("q", q, q.shape), ("k", k, k.shape), ("v", v, k.shape), *((n, t, q.shape) for n, t in same_as_q.items()),
-                           *((n, t, k.shape) for n, t in same_as_k.items())]:
-        if not t.is_cuda:
-            raise RuntimeError("emmyb200 kernels take CUDA tensors only (there is no CPU path)")
-        if t.shape != shape or t.dtype != q.dtype or t.device != q.device:
-            raise ValueError(f"{who}: {name} is {tuple(t.shape)} {t.dtype} on {t.device}; wanted {tuple(shape)} {q.dtype} on {q.device}")
-        if t.stride(3) != 1:
-            raise ValueError(f"{who}: the head dim of {name} must be contiguous")
-    if key_lens is not None and (key_lens.dtype != torch.int32 or key_lens.shape != q.shape[:1] or key_lens.device != q.device or not key_lens.is_contiguous()):
-        raise ValueError(f"{who}: key_lens is a contiguous int32 vector [batch] on {q.device}")
-    if bias_table is not None and (bias_table.dim() != 2 or bias_table.shape[1] != q.shape[1] or bias_table.device != q.device
-                                   or bias_table.dtype not in (torch.float32, torch.float16, torch.bfloat16)):
-        raise ValueError(f"{who}: bias_table is a float [buckets, heads] tensor on {q.device}")
-
-
-def _heads_flags(who: str, causal: bool, align: str) -> int:
-    if align not in ("start", "end"):
-        raise ValueError(f"{who}: align is 'start' or 'end'")
-    return (HEADS_CAUSAL if causal else 0) | (HEADS_ALIGN_END if align == "end" else 0)
+    if workspace is not None and (workspace[2] != torch.uint8 or workspace[3] != device or not dense(workspace) or math.prod(workspace[0]) < need):
+        raise ValueError(f"{who}: workspace is a contiguous uint8 tensor of at least {need} elements on {device}")
+    return desc, ctypes.byref(desc), need
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-class _On:
-    """The tensors' device and the launch's stream made current: what is allocated inside belongs to that stream."""
+class _Switched:
+    """The tensors' device and the launch's stream made current where they are not: what is allocated meanwhile belongs to
+    that stream. `handle` is the stream's."""
 
     def __init__(self, device, stream) -> None:
-        self.device, self.stream = device, stream
-
-    def __enter__(self) -> int:
         import torch
-        self.guards = [torch.cuda.device(self.device)] + ([torch.cuda.stream(self.stream)] if self.stream is not None else [])
+        self.guards = []
+        if device.type != "cuda":                   # refused with the reason when the call is checked
+            return
+        if torch.cuda.current_device() != device.index:
+            self.guards.append(torch.cuda.device(device))
+        if stream is not None:
+            self.guards.append(torch.cuda.stream(stream))
         for g in self.guards:
             g.__enter__()
-        return torch.cuda.current_stream().cuda_stream
+        self.handle = torch._C._cuda_getCurrentRawStream(device.index)
 
-    def __exit__(self, *error) -> None:
+    def back(self) -> None:
         for g in reversed(self.guards):
-            g.__exit__(*error)
-
-
-class _OnCurrent:
-    """The same where both are current already: nothing to switch."""
-
-    def __init__(self, handle: int) -> None:
-        self.handle = handle
-
-    def __enter__(self) -> int:
-        return self.handle
-
-    def __exit__(self, *error) -> None:
-        pass
-
-
-def _on(device, stream):
-    import torch
-    if stream is None and torch.cuda.current_device() == device.index:
-        return _OnCurrent(torch.cuda.current_stream(device.index).cuda_stream)
-    return _On(device, stream)
-
-
-def _heads_workspace(who: str, workspace, need: int, device):
-    import torch
-    if need == 0:
-        return None
-    if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=device)
-    if workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous() or workspace.numel() < need:
-        raise ValueError(f"{who}: workspace is a contiguous uint8 tensor of at least {need} elements on {device}")
-    return workspace
+            g.__exit__(None, None, None)
 
 
 def attention_heads(q, k, v, scale: float | None = None, causal: bool = False, align: str = "start", key_lens=None, bias_table=None,
@@ -744,26 +732,19 @@ def attention_heads(q, k, v, scale: float | None = None, causal: bool = False, a
     bucket(key position - query position), the buckets as `relative_runs(buckets, max_distance, bidirectional)`. A row that
     sees no key gives o = 0 and lse = -inf."""
     import torch
-    same = {} if out is None else {"out": out}
-    _heads_call("attention_heads", q, k, v, key_lens, bias_table, same, {})
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:3] or lse.device != q.device or not lse.is_contiguous()):
-        raise ValueError("attention_heads: lse is a contiguous float32 [batch, heads, seq_q] tensor")
-    with _on(q.device, stream) as handle:
+    at = _Switched(q.device, stream)
+    try:
         out = torch.empty_like(q) if out is None else out
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if lse is None else lse
-        desc, need = _heads_desc(False, dtype_code(q), _heads_flags("attention_heads", causal, align), tuple(q.shape), tuple(k.shape),
-                                 tuple(t.stride()[:3] for t in (q, k, v, out)), q.shape[3] ** -0.5 if scale is None else float(scale),
-                                 _heads_bias(bias_table, max_distance, bidirectional))
-        workspace = _heads_workspace("attention_heads", workspace, need, q.device)
-        check(library().emmyb200_attention_heads_fwd(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lens), _ptr(bias_table),
-                                                     out.data_ptr(), lse.data_ptr(), _ptr(workspace), need, handle))
+        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if lse is None else lse
+        desc, ref, need = _heads_plan("attention_heads", False, scale, causal, align, max_distance, bidirectional, _layout(key_lens), _layout(bias_table),
+                                      _layout(lse), None, _layout(workspace), _layout(q), _layout(k), _layout(v), _layout(out))
+        if need and workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        check(library().emmyb200_attention_heads_fwd(ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lens), _ptr(bias_table), out.data_ptr(),
+                                                     lse.data_ptr(), _ptr(workspace), need, at.handle))
+    finally:
+        at.back()
     return out, lse
-
-
-def _heads_bias(table, max_distance: int, bidirectional: bool):
-    if table is None:
-        return None
-    return dtype_code(table), tuple(table.stride()), table.shape[0], int(max_distance), bool(bidirectional)
 
 
 def attention_heads_backward(do, q, k, v, o, lse, scale: float | None = None, causal: bool = False, align: str = "start", key_lens=None,
@@ -774,27 +755,23 @@ def attention_heads_backward(do, q, k, v, o, lse, scale: float | None = None, ca
     lse. The gradients of shared key heads are summed over their query heads, dtable over the batch; gradients of keys
     behind key_lens are zero. Results do not depend on the order in which the blocks run."""
     import torch
-    who = "attention_heads_backward"
-    _heads_call(who, q, k, v, key_lens, bias_table, {"do": do, "o": o, **({} if dq is None else {"dq": dq})},
-                {n: t for n, t in (("dk", dk), ("dv", dv)) if t is not None})
-    if lse.dtype != torch.float32 or lse.shape != q.shape[:3] or lse.device != q.device or not lse.is_contiguous():
-        raise ValueError(f"{who}: lse is the contiguous float32 [batch, heads, seq_q] tensor of the forward")
-    if dtable is not None and (bias_table is None or dtable.shape != bias_table.shape or dtable.dtype != bias_table.dtype or dtable.device != q.device
-                               or not dtable.is_contiguous()):
-        raise ValueError(f"{who}: dtable is a contiguous tensor like bias_table")
-    with _on(q.device, stream) as handle:
+    at = _Switched(q.device, stream)
+    try:
         dq = torch.empty_like(q) if dq is None else dq
         dk = torch.empty_like(k) if dk is None else dk
         dv = torch.empty_like(v) if dv is None else dv
         if bias_table is not None and dtable is None:
             dtable = torch.empty(bias_table.shape, dtype=bias_table.dtype, device=q.device)
-        desc, need = _heads_desc(True, dtype_code(q), _heads_flags(who, causal, align), tuple(q.shape), tuple(k.shape),
-                                 tuple(t.stride()[:3] for t in (q, k, v, o, do, dq, dk, dv)), q.shape[3] ** -0.5 if scale is None else float(scale),
-                                 _heads_bias(bias_table, max_distance, bidirectional))
-        workspace = _heads_workspace(who, workspace, need, q.device)
-        check(library().emmyb200_attention_heads_bwd(ctypes.byref(desc), do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+        desc, ref, need = _heads_plan("attention_heads_backward", True, scale, causal, align, max_distance, bidirectional, _layout(key_lens),
+                                      _layout(bias_table), _layout(lse), _layout(dtable), _layout(workspace), _layout(q), _layout(k), _layout(v), _layout(o),
+                                      _layout(do), _layout(dq), _layout(dk), _layout(dv))
+        if need and workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        check(library().emmyb200_attention_heads_bwd(ref, do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
                                                      _ptr(key_lens), _ptr(bias_table), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable),
-                                                     _ptr(workspace), need, handle))
+                                                     _ptr(workspace), need, at.handle))
+    finally:
+        at.back()
     return (dq, dk, dv) if bias_table is None else (dq, dk, dv, dtable)
 
 

@@ -153,6 +153,14 @@ def test_forward_and_backward(shape, causal, dtype, cuda):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("causal,align", [(False, "start"), (True, "start"), (True, "end")])
+def test_more_tiles_than_SMs(causal, align, d, dtype, cuda):
+    """Several waves of blocks, and the CUDA-core kernels' larger tiles, with everything at once."""
+    Case(cuda, dtype, 5, 16, 8, 150, 210, d, causal=causal, align=align, lens=[210, 100, 64, 1, 199], buckets=32, rows_first=True, seed=d).run()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("bidirectional,causal", [(True, False), (False, True), (False, False), (True, True)])
 @pytest.mark.parametrize("b,h,hk,sq,sk,d,buckets,max_distance", [
     (2, 4, 2, 100, 130, 64, 32, 128), (1, 2, 2, 300, 300, 128, 8, 64), (1, 2, 1, 513, 400, 64, 128, 200), (3, 2, 2, 1, 200, 128, 32, 128),
