@@ -39,7 +39,8 @@ struct BwdParams {
     HeadsGrads g;
     MapAt q_at, k_at, v_at, do_at, dq_at, dk_at, dv_at;
     int q_tiles, k_tiles;
-    int chunk_dkv, chunk_dq;            // of units, see work_item
+    WorkOrder order_dkv, order_dq;
+    FastDiv by_heads, by_kv_heads, by_group;
     int dkv_blocks;                     // blocks from here on work on dQ
     unsigned long long wait_limit_ns;
     uint32_t* status;
@@ -146,9 +147,9 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const WorkItem work = work_item(item, p.h.batch * p.h.kv_heads, p.k_tiles, p.chunk_dkv);
+    const WorkItem work = p.order_dkv(item);
     const int kt = work.tile, bk = work.unit;                   // causal: the first key tiles see the most queries
-    const int b = bk / p.h.kv_heads, hk = bk % p.h.kv_heads;
+    const int b = p.by_kv_heads(bk), hk = bk - b * p.h.kv_heads;
     const int key0 = kt * kTile;
     const int n_keys = heads_key_count(p.h, b), offset = heads_offset(p.h, n_keys);
     const int q_tiles = (p.h.seq_q + kHalf - 1) / kHalf;
@@ -214,7 +215,7 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
             v_norm = __ldg(p.g.amax + (int64_t)p.h.batch * p.h.kv_heads + bk);
         }
     }
-    if constexpr (BIAS) load_runs(bias, p.h);
+    if constexpr (BIAS) load_runs(bias, p.h, warp, kBwdThreads / 32, lane);
     if (warp == 1) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
         ptx::tmem_relinquish();
@@ -430,7 +431,7 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
                     ptx::tma_store_4d(x ? &map_dk : &map_dv, tile + c * (kTile * 128), c * 64, key0, hk * (x ? p.dk_at.head : p.dv_at.head),
                                       b * (x ? p.dk_at.batch : p.dv_at.batch));
                 ptx::tma_store_commit();
-                ptx::tma_store_wait<0>();
+                ptx::tma_store_wait_read<0>();     // shared memory has been read; the grid's end covers the writes
             }
         }
     }
@@ -484,9 +485,9 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const WorkItem work = work_item(item, p.h.batch * p.h.heads, p.q_tiles, p.chunk_dq);
+    const WorkItem work = p.order_dq(item);
     const int bh = work.unit, qt = p.h.causal ? p.q_tiles - 1 - work.tile : work.tile;
-    const int b = bh / p.h.heads, h = bh % p.h.heads, hk = h / p.h.group;
+    const int b = p.by_heads(bh), h = bh - b * p.h.heads, hk = p.by_group(h);
     const int row0 = qt * kTile;
     const int n_keys = heads_key_count(p.h, b), offset = heads_offset(p.h, n_keys);
     const int key_end = p.h.causal ? max(0, min(n_keys, min(row0 + kTile, p.h.seq_q) + offset)) : n_keys;
@@ -532,7 +533,7 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
         }
     }
     if constexpr (BIAS) {
-        load_runs(bias, p.h);
+        load_runs(bias, p.h, warp, kBwdThreads / 32, lane);
         if ((int)threadIdx.x < p.h.n_runs) bias.value[threadIdx.x] = run_bias;
     }
     if (warp == 1) {
@@ -788,7 +789,7 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
                 for (int c = 0; c < kChunks; ++c)               // rows behind seq_q are dropped
                     ptx::tma_store_4d(&map_dq, smem_base + c * (kTile * 128), c * 64, row0, h * p.dq_at.head, b * p.dq_at.batch);
                 ptx::tma_store_commit();
-                ptx::tma_store_wait<0>();
+                ptx::tma_store_wait_read<0>();     // shared memory has been read; the grid's end covers the writes
             }
             __syncwarp();
             if constexpr (BIAS) {
@@ -839,8 +840,11 @@ static int launch_bwd(BwdParams& p, cudaStream_t s) {
     const int64_t kv_ctas = (int64_t)h.batch * h.kv_heads * p.k_tiles, q_ctas = (int64_t)h.batch * h.heads * p.q_tiles;
     if (kv_ctas + q_ctas >= (1ll << 31)) return fail(EMMYB200_ERR_SHAPE, "attention_heads_bwd: the tiles exceed the grid limit");
     p.dkv_blocks = (int)kv_ctas;
-    p.chunk_dkv = chunk_units(h.causal != 0, (int64_t)h.batch * h.kv_heads, (int64_t)h.seq_q * D * 4 * h.group);
-    p.chunk_dq = chunk_units(h.causal != 0, (int64_t)h.batch * h.heads, (int64_t)h.seq_k * D * 4 / h.group);
+    p.order_dkv = work_order(h.causal != 0, (int64_t)h.batch * h.kv_heads, p.k_tiles, (int64_t)h.seq_q * D * 4 * h.group);
+    p.order_dq = work_order(h.causal != 0, (int64_t)h.batch * h.heads, p.q_tiles, (int64_t)h.seq_k * D * 4 / h.group);
+    p.by_heads = fast_div(h.heads);
+    p.by_kv_heads = fast_div(h.kv_heads);
+    p.by_group = fast_div(h.group);
     auto kernel = h.n_runs ? heads_bwd_kernel<D, BF16, true> : heads_bwd_kernel<D, BF16, false>;
     EMMY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<D>::kTotal));
     kernel<<<(unsigned)(kv_ctas + q_ctas), kBwdThreads, BwdSmem<D>::kTotal, s>>>(m, p);

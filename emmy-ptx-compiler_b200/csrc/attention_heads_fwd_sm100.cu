@@ -30,8 +30,9 @@ struct FwdParams {
     MapAt q_at, k_at, v_at, o_at;
     int packed;                         // rows of a tile: group x seq_q (1) or 128 queries of one head (0)
     int tiles;                          // query tiles per unit (batch entry and head, or key head when packed)
-    int chunk;                          // of units, see work_item
     int splits;                         // CTAs that share a tile's keys
+    WorkOrder order;
+    FastDiv by_splits, by_unit_heads, by_group;
     float* lse;
     float* part_o;                      // splits > 1: [split][row][D], rows as lse
     float2* part_ml;                    // [split][row]: maximum (log2 units), sum
@@ -101,13 +102,12 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int split = blockIdx.x % p.splits;
-    const int item = blockIdx.x / p.splits;
+    const int item = p.by_splits(blockIdx.x), split = blockIdx.x - item * p.splits;
     const int unit_heads = p.packed ? p.h.kv_heads : p.h.heads;
-    const WorkItem work = work_item(item, p.h.batch * unit_heads, p.tiles, p.chunk);
+    const WorkItem work = p.order(item);
     const int unit = work.unit, qt = p.h.causal ? p.tiles - 1 - work.tile : work.tile;
-    const int b = unit / unit_heads, hu = unit % unit_heads;
-    const int head0 = p.packed ? hu * p.h.group : hu, hk = p.packed ? hu : hu / p.h.group;
+    const int b = p.by_unit_heads(unit), hu = unit - b * unit_heads;
+    const int head0 = p.packed ? hu * p.h.group : hu, hk = p.packed ? hu : p.by_group(hu);
     const int row0 = qt * kTile;
     const int box_rows = p.packed ? p.h.group * p.h.seq_q : kTile;
     const int n_keys = heads_key_count(p.h, b), offset = heads_offset(p.h, n_keys);
@@ -149,7 +149,7 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if constexpr (BIAS) {
         float run_bias = 0.0f;
         if ((int)threadIdx.x < p.h.n_runs) run_bias = heads_run_bias(p.h, threadIdx.x, head0);
-        load_runs(bias, p.h);
+        load_runs(bias, p.h, warp, kFwdThreads / 32, lane);
         if ((int)threadIdx.x < p.h.n_runs) bias.value[threadIdx.x] = run_bias;
     }
     if (warp == 1) {
@@ -363,7 +363,7 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     for (int c = 0; c < kChunks; ++c)
                         ptx::tma_store_4d(&map_o, q_smem + c * (kTile * 128), c * 64, row0, head0 * p.o_at.head, b * p.o_at.batch);
                     ptx::tma_store_commit();
-                    ptx::tma_store_wait<0>();
+                    ptx::tma_store_wait_read<0>();     // shared memory has been read; the grid's end covers the writes
                 }
             }
         }
@@ -432,7 +432,11 @@ static int launch(FwdParams& p, const FwdPlan& plan, const void* Q, const void* 
     EMMY_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p.status), g_fwd_status));
     const int64_t ctas = (int64_t)p.h.batch * (plan.packed ? p.h.kv_heads : p.h.heads) * p.tiles * p.splits;
     if (ctas >= (1ll << 31)) return fail(EMMYB200_ERR_SHAPE, "attention_heads_fwd: %lld tiles exceed the grid limit", (long long)ctas);
-    p.chunk = chunk_units(p.h.causal != 0, (int64_t)p.h.batch * (plan.packed ? p.h.kv_heads : p.h.heads), (int64_t)p.h.seq_k * D * 4 / (plan.packed ? 1 : p.h.group));
+    const int unit_heads = plan.packed ? p.h.kv_heads : p.h.heads;
+    p.order = work_order(p.h.causal != 0, (int64_t)p.h.batch * unit_heads, p.tiles, (int64_t)p.h.seq_k * D * 4 / (plan.packed ? 1 : p.h.group));
+    p.by_splits = fast_div(p.splits);
+    p.by_unit_heads = fast_div(unit_heads);
+    p.by_group = fast_div(p.h.group);
     auto kernel = p.h.n_runs ? heads_fwd_kernel<D, BF16, true> : heads_fwd_kernel<D, BF16, false>;
     EMMY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdSmem<D>::kTotal));
     kernel<<<(unsigned)ctas, kFwdThreads, FwdSmem<D>::kTotal, s>>>(mq, mk, mv, mo, p);
@@ -452,9 +456,16 @@ FwdPlan heads_fwd_plan(const HeadsParams& p) {
     plan.packed = p.group > 1 && (int64_t)p.group * p.seq_q <= heads::kTile && p.n_runs == 0 && p.q_s[1] != 0;
     plan.tiles = plan.packed ? 1 : (p.seq_q + heads::kTile - 1) / heads::kTile;
     const int64_t items = (int64_t)p.batch * (plan.packed ? p.kv_heads : p.heads) * plan.tiles;
+    // Splitting the keys costs a second launch and a set-up per CTA: worth it while there is less than one tile per SM (256 tiles
+    // of 64 key tiles each: 152 us whole, 171 us in two; 32 tiles: 126 us whole, 35 us in eight; 8 tiles: 121 us whole, 22 us in
+    // sixteen). Then as many CTAs as are resident at once, of at least four key tiles each, none of them shorter than it has to be.
     const int64_t key_tiles = (p.seq_k + heads::kTile - 1) / heads::kTile, slots = 2 * sm_count();
     plan.splits = 1;
-    if (items < slots) plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>((slots + items - 1) / items, key_tiles / 2));
+    if (items < sm_count()) {
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(slots / items, key_tiles / 4));
+        const int64_t each = (key_tiles + most - 1) / most;
+        plan.splits = (int)((key_tiles + each - 1) / each);
+    }
     plan.rows = (int64_t)p.batch * p.heads * p.seq_q;
     return plan;
 }

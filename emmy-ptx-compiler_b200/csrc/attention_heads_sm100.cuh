@@ -112,16 +112,17 @@ struct NearRuns {
         count = span <= kNear ? span : 0;
     }
 };
-// The part of the shared tables that does not depend on the head: thread r fills in run r.
-__device__ __forceinline__ void load_runs(BiasShared& s, const HeadsParams& p) {
-    const int r = threadIdx.x;
-    if (r >= p.n_runs) return;
+// The part of the shared tables that does not depend on the head: a warp per run, a lane per distance (a thread per run took 2000
+// cycles of a CTA's set-up for 32 runs within 128).
+__device__ __forceinline__ void load_runs(BiasShared& s, const HeadsParams& p, int warp, int warps, int lane) {
     const NearRuns near(p);
-    const int mine = p.run_first[r];
-    s.first[r] = mine;
-    if (near.count) {
-        const int to = r + 1 == p.n_runs ? near.count : p.run_first[r + 1] - near.first;
-        for (int i = r == 0 ? 0 : mine - near.first; i < to; ++i) s.near_run[i] = (uint8_t)r;
+    for (int r = warp; r < p.n_runs; r += warps) {
+        const int mine = p.run_first[r];
+        if (lane == 0) s.first[r] = mine;
+        if (near.count) {
+            const int to = r + 1 == p.n_runs ? near.count : p.run_first[r + 1] - near.first;
+            for (int i = (r == 0 ? 0 : mine - near.first) + lane; i < to; i += 32) s.near_run[i] = (uint8_t)r;
+        }
     }
 }
 struct WarpBias {
@@ -162,19 +163,36 @@ struct WarpBias {
 // longest tiles run alone (16 units of 2048 keys on 148 SMs: 184 us against 118). But CTAs that run at the same time should share
 // what they stream, so the units are taken in chunks whose streamed operands fit in a third of L2, each chunk longest first. chunk = 1: unit by
 // unit (tiles of equal length).
+// Division of 0 <= n < 2^31 by a number known at launch: a division instruction sequence takes some 150 cycles, a CTA's place in the work seven.
+struct FastDiv {
+    uint32_t mul, shift;
+    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+};
+inline FastDiv fast_div(int64_t d) {
+    uint32_t shift = 0;
+    while ((1ll << shift) < d) ++shift;
+    return {(uint32_t)((((1ull << shift) - (uint64_t)d) << 32) / (uint64_t)d + 1), shift};
+}
 struct WorkItem {
     int unit, tile;                     // tile: 0 is the longest
 };
-__device__ __forceinline__ WorkItem work_item(int item, int units, int tiles, int chunk) {
-    const int c = item / (chunk * tiles), in_chunk = item - c * chunk * tiles;
-    const int width = min(chunk, units - c * chunk);
-    return {c * chunk + in_chunk % width, in_chunk / width};
-}
+struct WorkOrder {
+    int units, tiles, chunk;
+    FastDiv per_chunk, width, last_width;       // chunk * tiles; units of a chunk; of the last one
+    __device__ __forceinline__ WorkItem operator()(int item) const {
+        const int c = per_chunk(item), in_chunk = item - c * chunk * tiles;
+        const bool last = (c + 1) * chunk > units;
+        const int w = last ? units - c * chunk : chunk, tile = last ? last_width(in_chunk) : width(in_chunk);
+        return {c * chunk + in_chunk - tile * w, tile};
+    }
+};
 // `bytes`: streamed by one unit's tiles.
-inline int chunk_units(bool causal, int64_t units, int64_t bytes) {
-    if (!causal) return 1;
+inline WorkOrder work_order(bool causal, int64_t units, int64_t tiles, int64_t bytes) {
     const int64_t fit = (42ll << 20) / (bytes > 0 ? bytes : 1);
-    return (int)(fit < 1 ? 1 : fit > units ? units : fit);
+    int64_t chunk = !causal || fit < 1 ? 1 : fit > units ? units : fit;
+    if (chunk * tiles >= (1ll << 31)) chunk = 1;
+    const int64_t rest = units % chunk;
+    return {(int)units, (int)tiles, (int)chunk, fast_div(chunk * tiles), fast_div(chunk), fast_div(rest ? rest : chunk)};
 }
 
 // ---- strided operands ---------------------------------------------------------------------------------------------------
