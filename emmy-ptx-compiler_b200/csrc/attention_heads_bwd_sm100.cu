@@ -74,24 +74,17 @@ __device__ __forceinline__ float ds_scale(float do_norm, float v_norm) {
     return __int_as_float(((int)fminf(fmaxf(floorf(-log2f(bound)), -100.0f), 100.0f) + 127) << 23);
 }
 
-// A row of a strided operand on its way into tensor memory, as the A operand of a product: element pairs in columns, COLS of
-// them. Loaded before the CTA has its tensor memory, stored after. Rows that do not exist are zeros.
-template <int COLS>
-__device__ __forceinline__ void load_row(uint4 (&v)[COLS / 4], const uint16_t* src, bool exists) {
+// A row of a 128-row tile in shared memory (pieces of 128 rows x 64 elements, 128-byte swizzle) into tensor memory, as the A operand of a
+// product: D / 2 columns of element pairs. (Threads reading their rows from global memory instead took 7000 cycles of a CTA's set-up.)
+template <int D>
+__device__ __forceinline__ void row_to_tmem(uint32_t taddr, uint32_t tile, int row) {
 #pragma unroll
-    for (int i = 0; i < COLS / 4; ++i) v[i] = exists ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-}
-template <int COLS>
-__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const uint4 (&v)[COLS / 4]) {
-#pragma unroll
-    for (int i = 0; i < COLS / 16; ++i) {
+    for (int i = 0; i < D / 32; ++i) {          // 32 elements
         uint32_t r[16];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            r[4 * k] = v[4 * i + k].x;
-            r[4 * k + 1] = v[4 * i + k].y;
-            r[4 * k + 2] = v[4 * i + k].z;
-            r[4 * k + 3] = v[4 * i + k].w;
+            const int piece = (i % 2) * 4 + k;
+            ptx::ld_shared_16B(tile + (i / 2) * (kTile * 128) + row * 128 + ((piece ^ (row & 7)) << 4), r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
         }
         ptx::tmem_st_32x32b_x16(taddr + 16 * i, r);
     }
@@ -140,7 +133,7 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
     auto do_smem = [&](int s) { return smem_base + (4 + kStages + s) * S::kStage; };
     const uint32_t rows_smem = smem_base + S::kRowsOffset;
     const uint32_t bar_base = smem_base + S::kBarOffset;
-    const uint32_t kv_ready = bar_base, acc_full = bar_base + 16, s_full = bar_base + 24 /* per group */, dp_full = bar_base + 40,
+    const uint32_t kv_full = bar_base, kv_ready = kKvInTmem ? bar_base + 8 : kv_full, acc_full = bar_base + 16, s_full = bar_base + 24 /* per group */, dp_full = bar_base + 40,
                    p_ready = bar_base + 56, ds_ready = bar_base + 72, staged = bar_base + 104, full = bar_base + 128, empty = full + 8 * kStages;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 120);
     volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -178,7 +171,8 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
         ++load_it;
     };
     if (threadIdx.x == 0) {
-        ptx::mbar_init(kv_ready, kKvInTmem ? 8 : 1); ptx::mbar_init(acc_full, 1);
+        ptx::mbar_init(kv_full, 1); ptx::mbar_init(acc_full, 1);
+        if (kKvInTmem) ptx::mbar_init(kv_ready, 8);
         for (int x = 0; x < 2; ++x) {
             ptx::mbar_init(s_full + 8 * x, 1); ptx::mbar_init(dp_full + 8 * x, 1); ptx::mbar_init(p_ready + 8 * x, 4); ptx::mbar_init(ds_ready + 8 * x, 4); ptx::mbar_init(staged + 8 * x, 4);
         }
@@ -188,13 +182,11 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
         *abort_flag = 0;
         ptx::mbar_fence_init();
         if (n_it > 0) {                                         // the first loads fly while the CTA sets itself up
-            if (!kKvInTmem) {
-                ptx::mbar_arrive_expect_tx(kv_ready, 4 * S::kStage);
+            ptx::mbar_arrive_expect_tx(kv_full, 4 * S::kStage);
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c) {
-                    ptx::tma_load_4d(k_smem + c * (kTile * 128), &map_k, kv_ready, c * 64, key0, hk * p.k_at.head, b * p.k_at.batch);
-                    ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, kv_ready, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
-                }
+            for (int c = 0; c < kChunks; ++c) {
+                ptx::tma_load_4d(k_smem + c * (kTile * 128), &map_k, kv_full, c * 64, key0, hk * p.k_at.head, b * p.k_at.batch);
+                ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, kv_full, c * 64, key0, hk * p.v_at.head, b * p.v_at.batch);
             }
             load_stage(load_s, load_gi, load_qt);
             advance();
@@ -202,18 +194,10 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
     }
     const int x = (warp - 2) >> 2;                              // group of the warps 2 to 9
     const int key = key0 + (warp & 3) * 32 + lane;
-    // loads from here to the barrier are in flight together
-    uint4 a_row[D / 8];
     float do_norm = 0.0f, v_norm = 0.0f;
-    if (warp >= 2 && n_it > 0) {
-        if constexpr (kKvInTmem)                                // group 0 brings K to tensor memory, group 1 V
-            load_row<D / 2>(a_row, x ? static_cast<const uint16_t*>(p.g.v) + b * p.h.v_s[0] + hk * p.h.v_s[1] + key * p.h.v_s[2]
-                                     : static_cast<const uint16_t*>(p.g.k) + b * p.h.k_s[0] + hk * p.h.k_s[1] + key * p.h.k_s[2],
-                            key < n_keys);
-        if (!BF16) {
-            do_norm = __ldg(p.g.amax + bk);
-            v_norm = __ldg(p.g.amax + (int64_t)p.h.batch * p.h.kv_heads + bk);
-        }
+    if (!BF16 && warp >= 2) {
+        do_norm = __ldg(p.g.amax + bk);
+        v_norm = __ldg(p.g.amax + (int64_t)p.h.batch * p.h.kv_heads + bk);
     }
     if constexpr (BIAS) load_runs(bias, p.h, warp, kBwdThreads / 32, lane);
     if (warp == 1) {
@@ -238,18 +222,20 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
         // ---- MMA issuer: S(0) dP(0) S(1) dP(1) | dV(i) S(i+2) dK(i) dP(i+2) | ... ----------------------------------
         if (n_it > 0) {
             const uint32_t lead = ptx::elect_lead();
+            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            const int tiles = __shfl_sync(0xffffffffu, n_it, 0);
             auto s_product = [&](int it, int s) {
-                if constexpr (kKvInTmem) Mma::scores_ts(lead, tmem_base + kColS + 64 * (it & 1), tmem_base + kColK, q_smem(s));
-                else Mma::scores_ss(lead, tmem_base + kColS + 64 * (it & 1), k_smem, q_smem(s));
+                if constexpr (kKvInTmem) Mma::scores_ts(lead, tmem + kColS + 64 * (it & 1), tmem + kColK, q_smem(s));
+                else Mma::scores_ss(lead, tmem + kColS + 64 * (it & 1), k_smem, q_smem(s));
                 ptx::mma_commit_lead(lead, s_full + 8 * (it & 1));
             };
             auto dp_product = [&](int it, int s) {
-                if constexpr (kKvInTmem) Mma::scores_ts(lead, tmem_base + kColDP + 64 * (it & 1), tmem_base + kColV, do_smem(s));
-                else Mma::scores_ss(lead, tmem_base + kColDP + 64 * (it & 1), v_smem, do_smem(s));
+                if constexpr (kKvInTmem) Mma::scores_ts(lead, tmem + kColDP + 64 * (it & 1), tmem + kColV, do_smem(s));
+                else Mma::scores_ss(lead, tmem + kColDP + 64 * (it & 1), v_smem, do_smem(s));
                 ptx::mma_commit_lead(lead, dp_full + 8 * (it & 1));
             };
             bool ok = warp_spin(wctx, kv_ready, 0, 0x05030000u);
-            for (int it = 0; it < 2 && it < n_it && ok; ++it) {
+            for (int it = 0; it < 2 && it < tiles && ok; ++it) {
                 if (!(ok = warp_spin(wctx, full + 8 * it, 0, 0x05040000u | it))) break;
                 ptx::tc_fence_after_sync();
                 s_product(it, it);
@@ -257,17 +243,17 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
             }
             int s = 0, next = 2;                                // stages of tiles it and it + 2
             uint32_t next_phase = 0;
-            for (int it = 0; it < n_it && ok; ++it) {
+            for (int it = 0; it < tiles && ok; ++it) {
                 const uint32_t x64 = 64 * (it & 1), phase = (it >> 1) & 1;
-                const bool more = it + 2 < n_it;
+                const bool more = it + 2 < tiles;
                 if (more && !(ok = warp_spin(wctx, full + 8 * next, next_phase, 0x05050000u | (it & 0xffff)))) break;
                 if (!(ok = warp_spin(wctx, p_ready + 8 * (it & 1), phase, 0x05070000u | (it & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
-                Mma::grads(lead, tmem_base + kColDV, tmem_base + kColS + x64, do_smem(s), it == 0);
+                Mma::grads(lead, tmem + kColDV, tmem + kColS + x64, do_smem(s), it == 0);
                 if (more) s_product(it + 2, next);
                 if (!(ok = warp_spin(wctx, ds_ready + 8 * (it & 1), phase, 0x05080000u | (it & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
-                Mma::grads(lead, tmem_base + kColDK, tmem_base + kColDP + x64, q_smem(s), it == 0);
+                Mma::grads(lead, tmem + kColDK, tmem + kColDP + x64, q_smem(s), it == 0);
                 ptx::mma_commit_lead(lead, empty + 8 * s);
                 if (more) dp_product(it + 2, next);
                 if (++s == kStages) s = 0;
@@ -281,8 +267,9 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
         const int w = warp - 2, quarter = warp & 3;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_at = tmem_base + lane_base + kColS + x * 64, dp_at = tmem_base + lane_base + kColDP + x * 64;
-        if (kKvInTmem && n_it > 0) {
-            row_to_tmem<D / 2>(tmem_base + lane_base + (x ? kColV : kColK), a_row);
+        bool ok = true;
+        if (kKvInTmem && n_it > 0 && (ok = warp_wait(wctx, kv_full, 0, 0x05090000u))) {          // group 0 writes K to tensor memory, group 1 V
+            row_to_tmem<D>(tmem_base + lane_base + (x ? kColV : kColK), x ? v_smem : k_smem, quarter * 32 + lane);
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
             __syncwarp();
@@ -290,7 +277,6 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
         }
         const float g_scale = BF16 ? 1.0f : ds_scale(do_norm, v_norm);
         const float2 g2 = make_float2(g_scale, g_scale);
-        bool ok = true;
         WarpBias wb(p.h);
         float* value = reinterpret_cast<float*>(smem_gen + S::kSumsOffset) + w * kHeadsMaxRuns;
         int bias_head = -1;
@@ -478,7 +464,7 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
     auto k_smem = [&](int s) { return smem_base + s * S::kStage; };
     auto v_smem = [&](int s) { return smem_base + (kStages + s) * S::kStage; };
     const uint32_t bar_base = smem_base + S::kBarOffset;
-    const uint32_t a_ready = bar_base, acc_full = bar_base + 8, s_full = bar_base + 16 /* per group */, dp_full = bar_base + 32, ds_ready = bar_base + 48, s_free = bar_base + 64, staged = bar_base + 80,
+    const uint32_t a_ready = bar_base, a_full = bar_base + 96, acc_full = bar_base + 8, s_full = bar_base + 16 /* per group */, dp_full = bar_base + 32, ds_ready = bar_base + 48, s_free = bar_base + 64, staged = bar_base + 80,
                    full = bar_base + 128, empty = full + 8 * kStages;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 120);
     volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -503,7 +489,7 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
         }
     };
     if (threadIdx.x == 0) {
-        ptx::mbar_init(a_ready, 8); ptx::mbar_init(acc_full, 1); ptx::mbar_init(staged, 8);
+        ptx::mbar_init(a_ready, 8); ptx::mbar_init(a_full, 1); ptx::mbar_init(acc_full, 1); ptx::mbar_init(staged, 8);
         for (int x = 0; x < 2; ++x) {
             ptx::mbar_init(s_full + 8 * x, 1); ptx::mbar_init(dp_full + 8 * x, 1); ptx::mbar_init(ds_ready + 8 * x, 4); ptx::mbar_init(s_free + 8 * x, 4);
         }
@@ -512,18 +498,24 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
         }
         *abort_flag = 0;
         ptx::mbar_fence_init();
-        if (n_it > 0) load_stage(0, 0);                         // flies while the CTA sets itself up
+        if (n_it > 0) {                                         // these fly while the CTA sets itself up; Q and dO where the last two stages will be
+            ptx::mbar_arrive_expect_tx(a_full, 4 * S::kStage);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int r = 0; r < kTile; r += kHalf) {
+                    ptx::tma_load_4d(k_smem(kStages - 2) + c * (kTile * 128) + r * 128, &m.q, a_full, c * 64, row0 + r, h * p.q_at.head, b * p.q_at.batch);
+                    ptx::tma_load_4d(v_smem(kStages - 2) + c * (kTile * 128) + r * 128, &m.d_o, a_full, c * 64, row0 + r, h * p.do_at.head, b * p.do_at.batch);
+                }
+            load_stage(0, 0);
+        }
     }
     const int x = (warp - 2) >> 2;                              // group of the warps 2 to 9
     const int row = row0 + (warp & 3) * 32 + lane;
     // loads from here to the barrier are in flight together
-    uint4 a_row[D / 8];
     float nlse = 0.0f, ndelta = 0.0f, do_norm = 0.0f, v_norm = 0.0f, run_bias = 0.0f;
     if (BIAS && (int)threadIdx.x < p.h.n_runs) run_bias = heads_run_bias(p.h, threadIdx.x, h);
-    if (warp >= 2) {                                            // group 0 brings Q to tensor memory, group 1 dO
-        load_row<D / 2>(a_row, x ? static_cast<const uint16_t*>(p.g.d_o) + b * p.h.do_s[0] + h * p.h.do_s[1] + row * p.h.do_s[2]
-                                 : static_cast<const uint16_t*>(p.g.q) + b * p.h.q_s[0] + h * p.h.q_s[1] + row * p.h.q_s[2],
-                        row < p.h.seq_q);
+    if (warp >= 2) {
         const int64_t at_row = (int64_t)bh * p.g.pad_q + row;
         nlse = p.g.lse2[at_row];
         ndelta = p.g.delta[at_row];
@@ -551,6 +543,7 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
             int s = 1;
             uint32_t phase = 1;
             for (int it = 1; it < n_it; ++it) {
+                if (it == kStages - 2 && !bounded_wait(wctx, a_ready, 0, 0x06010000u)) break;          // Q and dO have left the last stages
                 if (!bounded_wait(wctx, empty + 8 * s, phase, 0x06010000u | (it & 0xffff))) break;
                 load_stage(s, it);
                 if (++s == kStages) { s = 0; phase ^= 1; }
@@ -561,16 +554,18 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
         // ---- MMA issuer: S(0) dP(0) S(1) dP(1) | S(i+2) dQ(i) dP(i+2) | ... ------------------------------------------
         if (n_it > 0) {
             const uint32_t lead = ptx::elect_lead();
+            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            const int tiles = __shfl_sync(0xffffffffu, n_it, 0);
             auto s_product = [&](int it, int s) {
-                Mma::scores_ts(lead, tmem_base + kColS + 64 * (it & 1), tmem_base + kColQ, k_smem(s));
+                Mma::scores_ts(lead, tmem + kColS + 64 * (it & 1), tmem + kColQ, k_smem(s));
                 ptx::mma_commit_lead(lead, s_full + 8 * (it & 1));
             };
             auto dp_product = [&](int it, int s) {
-                Mma::scores_ts(lead, tmem_base + kColDP + 64 * (it & 1), tmem_base + kColDO, v_smem(s));
+                Mma::scores_ts(lead, tmem + kColDP + 64 * (it & 1), tmem + kColDO, v_smem(s));
                 ptx::mma_commit_lead(lead, dp_full + 8 * (it & 1));
             };
             bool ok = warp_spin(wctx, a_ready, 0, 0x06030000u);
-            for (int it = 0; it < 2 && it < n_it && ok; ++it) {
+            for (int it = 0; it < 2 && it < tiles && ok; ++it) {
                 if (!(ok = warp_spin(wctx, full + 8 * it, 0, 0x06040000u | it))) break;
                 ptx::tc_fence_after_sync();
                 s_product(it, it);
@@ -578,9 +573,9 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
             }
             int s = 0, next = 2;                                // stages of tiles it and it + 2
             uint32_t next_phase = 0;
-            for (int it = 0; it < n_it && ok; ++it) {
+            for (int it = 0; it < tiles && ok; ++it) {
                 const uint32_t phase = (it >> 1) & 1;
-                const bool more = it + 2 < n_it;
+                const bool more = it + 2 < tiles;
                 if (more) {
                     if (!(ok = warp_spin(wctx, full + 8 * next, next_phase, 0x06050000u | (it & 0xffff)))) break;
                     // S(it) is in registers: its columns are free
@@ -590,7 +585,7 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
                 }
                 if (!(ok = warp_spin(wctx, ds_ready + 8 * (it & 1), phase, 0x06070000u | (it & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
-                Mma::grads(lead, tmem_base + kColDQ, tmem_base + kColDP + 64 * (it & 1), k_smem(s), it == 0);
+                Mma::grads(lead, tmem + kColDQ, tmem + kColDP + 64 * (it & 1), k_smem(s), it == 0);
                 ptx::mma_commit_lead(lead, empty + 8 * s);
                 if (more) dp_product(it + 2, next);
                 if (++s == kStages) s = 0;
@@ -604,8 +599,9 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
         const int w = warp - 2, quarter = warp & 3;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_at = tmem_base + lane_base + kColS + x * 64, dp_at = tmem_base + lane_base + kColDP + x * 64;
-        if (n_it > 0) {
-            row_to_tmem<D / 2>(tmem_base + lane_base + (x ? kColDO : kColQ), a_row);
+        bool ok = true;
+        if (n_it > 0 && (ok = warp_wait(wctx, a_full, 0, 0x06020000u))) {        // group 0 writes Q to tensor memory, group 1 dO
+            row_to_tmem<D>(tmem_base + lane_base + (x ? kColDO : kColQ), x ? v_smem(kStages - 2) : k_smem(kStages - 2), quarter * 32 + lane);
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
             __syncwarp();
@@ -617,7 +613,6 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
         const bool want_bias = BIAS && p.g.dtable != nullptr;
         float* sums = reinterpret_cast<float*>(smem_gen + S::kSumsOffset) + w * kHeadsMaxRuns;      // this warp's, by run
         RunSums rs{0.0f, 0};
-        bool ok = true;
         WarpBias wb(p.h);
         if constexpr (BIAS) {
             for (int r = lane; r < p.h.n_runs; r += 32) sums[r] = 0.0f;

@@ -179,11 +179,13 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             constexpr uint32_t idesc_o = ptx::mma_idesc_f16(BF16, false, true, kTile, D);
             constexpr uint32_t hi = ptx::smem_desc_sw128_hi(1024);
             const uint32_t lead = ptx::elect_lead();
-            const uint32_t s_tmem = tmem_base, o_tmem = tmem_base + kColO;
             const uint32_t q_lo = ptx::smem_desc_sw128_lo(q_smem, 16), k_lo = ptx::smem_desc_sw128_lo(k_smem, 16), v_lo = ptx::smem_desc_sw128_lo(v_smem, kTile * 128);
-            auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) { return __all_sync(0xffffffffu, bounded_wait(wctx, bar, parity, code)) != 0; };
-            bool ok = kv_tiles == 0 || wait(q_full, 0, 0x04030000u);
-            for (int j = 0; j < kv_tiles && ok; ++j) {
+            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            const int tiles = __shfl_sync(0xffffffffu, kv_tiles, 0);
+            auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) { return warp_spin(wctx, bar, parity, code); };
+            const uint32_t s_tmem = tmem, o_tmem = tmem + kColO;
+            bool ok = tiles == 0 || wait(q_full, 0, 0x04030000u);
+            for (int j = 0; j < tiles && ok; ++j) {
                 const uint32_t ph = j & 1;
                 if (!(ok = wait(k_full, ph, 0x04040000u | (j & 0xffff)))) break;
                 ptx::tc_fence_after_sync();

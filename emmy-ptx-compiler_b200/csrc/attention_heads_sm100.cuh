@@ -58,35 +58,31 @@ __device__ __forceinline__ uint32_t operand_pair(float2 v) {
 
 // ---- waits of a whole warp ---------------------------------------------------------------------------------------------------
 // One poll by all lanes and a vote is the common case and costs some 50 cycles less than a loop per lane around it (the
-// issuing warp makes four waits per tile: with the per-lane form they took longer than the products). The loops behind it keep
-// the limit and the abort flag of bounded_wait / bounded_spin; the answer is the warp's.
-__device__ __noinline__ inline bool warp_wait_slow(volatile uint32_t* abort_flag, uint32_t* status, uint64_t limit_ns, uint32_t bar, uint32_t parity, uint32_t code, bool spin) {
+// issuing warp makes three or four waits per tile: with the per-lane form they took longer than the products). The limit and the
+// abort flag are those of bounded_wait / bounded_spin; the answer is the warp's. All of it is inlined: across a call the compiler keeps
+// nothing in uniform registers, and every operand of every product was moved there again (64 cycles per product instruction against 43).
+template <bool PARK>
+__device__ __forceinline__ bool warp_poll(const WaitCtx& ctx, uint32_t bar, uint32_t parity, uint32_t code) {
+    if (__all_sync(0xffffffffu, ptx::mbar_test_wait(bar, parity))) return true;
     uint64_t t0 = 0;
     for (uint32_t n = 1;; ++n) {
-        const bool done = spin ? ptx::mbar_test_wait(bar, parity) : ptx::mbar_try_wait(bar, parity);
-        if (__all_sync(0xffffffffu, done)) return true;
-        if ((n & (spin ? 63u : 15u)) == 0) {
+        if (__all_sync(0xffffffffu, PARK ? ptx::mbar_try_wait(bar, parity) : ptx::mbar_test_wait(bar, parity))) return true;
+        if ((n & (PARK ? 15u : 63u)) == 0) {
             const uint64_t now = ptx::global_timer_ns();
             if (t0 == 0) t0 = now;
-            const bool late = now - t0 > limit_ns;
+            const bool late = now - t0 > ctx.limit_ns;
             if (late) {
-                atomicCAS(status, 0u, code);
-                *abort_flag = 1;
+                atomicCAS(ctx.status_word, 0u, code);
+                *ctx.abort_flag = 1;
             }
-            if (__any_sync(0xffffffffu, late || *abort_flag != 0)) return false;
+            if (__any_sync(0xffffffffu, late || *ctx.abort_flag != 0)) return false;
         }
     }
 }
 // Parks the warp while it waits.
-__device__ __forceinline__ bool warp_wait(const WaitCtx& ctx, uint32_t bar, uint32_t parity, uint32_t code) {
-    if (__all_sync(0xffffffffu, ptx::mbar_test_wait(bar, parity))) return true;
-    return warp_wait_slow(ctx.abort_flag, ctx.status_word, ctx.limit_ns, bar, parity, code, false);
-}
+__device__ __forceinline__ bool warp_wait(const WaitCtx& ctx, uint32_t bar, uint32_t parity, uint32_t code) { return warp_poll<true>(ctx, bar, parity, code); }
 // Polls without parking (the issuing warp).
-__device__ __forceinline__ bool warp_spin(const WaitCtx& ctx, uint32_t bar, uint32_t parity, uint32_t code) {
-    if (__all_sync(0xffffffffu, ptx::mbar_test_wait(bar, parity))) return true;
-    return warp_wait_slow(ctx.abort_flag, ctx.status_word, ctx.limit_ns, bar, parity, code, true);
-}
+__device__ __forceinline__ bool warp_spin(const WaitCtx& ctx, uint32_t bar, uint32_t parity, uint32_t code) { return warp_poll<false>(ctx, bar, parity, code); }
 
 // ---- the bias --------------------------------------------------------------------------------------------------------
 // A warp works on 32 x 64 blocks of scores, which span 95 distances. Where they all fall into one run (far from the
