@@ -104,8 +104,8 @@ struct NearRuns {
     int first, count;                   // count 0: not used
     __device__ __forceinline__ NearRuns(const HeadsParams& p) {
         first = p.n_runs > 1 ? p.run_first[1] - 1 : 0;
-        const int span = p.n_runs > 1 ? p.run_first[p.n_runs - 1] - first + 1 : 1;
-        count = span <= kNear ? span : 0;
+        const long long span = p.n_runs > 1 ? (long long)p.run_first[p.n_runs - 1] - first + 1 : 1;
+        count = span <= kNear ? (int)span : 0;
     }
 };
 // The part of the shared tables that does not depend on the head: a warp per run, a lane per distance (a thread per run took 2000

@@ -328,6 +328,7 @@ int emmyb200_attention_fwd_allgather(int dtype, int flags, const void* Q, const 
  *     dtable[bucket][h] = sum of dS_ij over the batch and the pairs of that bucket
  * dtable: [buckets][heads] contiguous, bias_dtype, NULL when not wanted. All gradients are overwritten, those of keys
  * behind key_lens with zeros. No atomics on values: results do not depend on the order in which blocks finish.
+ * No output may overlap an input or another output.
  *
  * Workspace: emmyb200_attention_heads_workspace_bytes(desc, backward) bytes (0: none) of 256-byte aligned device memory,
  * contents irrelevant before, undefined after; -1 for a description the call would reject. Calls that may run at the same time

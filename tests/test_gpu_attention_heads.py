@@ -170,6 +170,57 @@ def test_bias(b, h, hk, sq, sk, d, buckets, max_distance, bidirectional, causal,
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_bias_over_more_distances_than_the_table_holds(dtype, cuda):
+    """Distances spread over more than 4096: the runs are searched instead of looked up."""
+    Case(cuda, dtype, 1, 2, 1, 700, 650, 64, buckets=64, max_distance=9000, seed=31).run()
+    Case(cuda, dtype, 2, 2, 2, 150, 5000, 128, causal=True, align="end", lens=[5000, 4700], buckets=32, max_distance=4500, bidirectional=False, seed=32).run()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,sq,buckets", [(4, 2, 1, 0), (4, 1, 3, 0), (2, 2, 2, 32)])
+def test_tokens_against_long_caches(heads, kv_heads, sq, buckets, dtype, cuda):
+    """Few rows against 200003 keys: the keys are split over many CTAs, some of which lie behind a short request's last key."""
+    Case(cuda, dtype, 3, heads, kv_heads, sq, 200003, 64, causal=True, align="end", lens=[200003, 1, 130000], buckets=buckets, seed=33).run()
+
+
+def test_runs_of_the_caller(cuda, lib):
+    """The C entry points take any runs of distance: one run alone, and runs that name a bucket twice and leave one out."""
+    import ctypes
+    from emmyptx import runtime
+    c = Case(cuda, "bf16", 2, 2, 2, 150, 200, 64, buckets=4, seed=34)
+    lse = torch.empty(2, 2, 150, device=cuda)
+    o, dq, dk, dv = (torch.empty_like(x) for x in (c.q, c.q, c.k, c.v))
+    dtable = torch.empty_like(c.table)
+    for runs in ([(0, 2)], [(0, 1), (-100, 3), (-5, 0), (0, 3), (7, 1)], [(0, 0), (-(1 << 30), 1), (1 << 30, 3)]):
+        d = runtime.HeadsDesc()
+        d.dtype, d.scale, d.bias_dtype, d.buckets, d.n_runs = runtime.BF16, c.scale, runtime.F32, 4, len(runs)
+        d.batch, d.heads, d.kv_heads, d.seq_q, d.seq_k, d.d = 2, 2, 2, 150, 200, 64
+        for n, x in (("q", c.q), ("k", c.k), ("v", c.v), ("o", o), ("do", c.do), ("dq", dq), ("dk", dk), ("dv", dv)):
+            getattr(d, f"{n}_stride")[:] = x.stride()[:3]
+        d.bias_stride[:] = c.table.stride()
+        d.run_first[:len(runs)], d.run_bucket[:len(runs)] = [r[0] for r in runs], [r[1] for r in runs]
+        ws = torch.empty(max(lib.emmyb200_attention_heads_workspace_bytes(ctypes.byref(d), 1), 256), dtype=torch.uint8, device=cuda)
+        stream = torch.cuda.current_stream().cuda_stream
+        assert lib.emmyb200_attention_heads_fwd(ctypes.byref(d), c.q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), None, c.table.data_ptr(), o.data_ptr(),
+                                                lse.data_ptr(), ws.data_ptr(), ws.numel(), stream) == 0
+        assert lib.emmyb200_attention_heads_bwd(ctypes.byref(d), c.do.data_ptr(), c.q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+                                                None, c.table.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dtable.data_ptr(), ws.data_ptr(),
+                                                ws.numel(), stream) == 0
+        dist = torch.arange(200, device=cuda)[None] - torch.arange(150, device=cuda)[:, None]
+        bucket = torch.full_like(dist, runs[0][1])
+        for first, b in runs[1:]:
+            bucket[dist >= first] = b
+        q, k, v, table = (x.double() for x in (c.q, c.k, c.v, c.table))
+        p = torch.softmax(q @ k.transpose(-1, -2) * c.scale + table.t()[:, bucket], -1)
+        ds = p * (c.do.double() @ v.transpose(-1, -2) - (c.do.double() * o.double()).sum(-1, keepdim=True))
+        want = torch.stack([ds[:, :, bucket == b].sum((0, 2)) for b in range(4)])
+        # one rounding of o and of p, and of the result: 2^-8 each in the 2-norm; dtable is fp32 throughout, its sums cancel to some 1e-3 of their terms
+        assert (o.double() - p @ v).norm() <= 3 * 2.0 ** -8 * (p @ v).norm()
+        assert (dtable.double() - want).abs().max() <= 1e-5 * ds.abs().sum()
+        assert all(torch.all(dtable[b] == 0) for b in range(4) if b not in [r[1] for r in runs])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("align", ["start", "end"])
 @pytest.mark.parametrize("buckets", [0, 32])
@@ -357,10 +408,11 @@ def test_another_stream_and_the_current_one(cuda):
         assert torch.equal(x, y) and torch.equal(x, z)
 
 
-def test_captured_and_replayed(cuda):
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_captured_and_replayed(dtype, cuda):
     """A step captured into a graph and replayed on new inputs, with a second captured graph beside it."""
     from emmyptx import runtime
-    cases = [Case(cuda, "bf16", 2, 4, 2, 150, 150, 64, lens=[150, 90], buckets=32, seed=s) for s in (1, 2)]
+    cases = [Case(cuda, dtype, 2, 4, 2, 150, 150, 64, lens=[150, 90], buckets=32, seed=s) for s in (1, 2)]
     graphs, outs = [], []
     for c in cases:
         def step():
@@ -375,7 +427,7 @@ def test_captured_and_replayed(cuda):
         with torch.cuda.graph(g):
             outs.append(step())
         graphs.append(g)
-    fresh = [Case(cuda, "bf16", 2, 4, 2, 150, 150, 64, lens=[20, 150], buckets=32, seed=s) for s in (3, 4)]
+    fresh = [Case(cuda, dtype, 2, 4, 2, 150, 150, 64, lens=[20, 150], buckets=32, seed=s) for s in (3, 4)]
     for c, f in zip(cases, fresh):
         for name in ("q", "k", "v", "do", "lens", "table"):
             getattr(c, name).copy_(getattr(f, name))
@@ -386,6 +438,25 @@ def test_captured_and_replayed(cuda):
         o, lse = runtime.attention_heads(f.q, f.k, f.v, **f.how)
         want = (o, lse, *runtime.attention_heads_backward(f.do, f.q, f.k, f.v, o, lse, **f.how))
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_two_streams_at_once(cuda):
+    """The same step on two streams without any order between them, several times over."""
+    from emmyptx import runtime
+    c = Case(cuda, "f16", 2, 8, 2, 500, 500, 64, causal=True, buckets=32, seed=41)
+
+    def step():
+        o, lse = runtime.attention_heads(c.q, c.k, c.v, **c.how)
+        return (o, lse, *runtime.attention_heads_backward(c.do, c.q, c.k, c.v, o, lse, **c.how))
+    want = step()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for g in got for x, y in zip(want, g))
 
 
 def test_offsets_beyond_32_bits(cuda):
