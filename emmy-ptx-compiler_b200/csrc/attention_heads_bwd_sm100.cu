@@ -52,8 +52,6 @@ struct BwdMaps {
 
 __device__ uint32_t g_bwd_status;
 
-constexpr int kHalf = 64;               // columns of a tile: rows of a stage
-
 template <int D>
 struct BwdSmem {
     static constexpr int kStage = kHalf * D * 2;
@@ -90,33 +88,6 @@ __device__ __forceinline__ void row_to_tmem(uint32_t taddr, uint32_t tile, int r
     }
 }
 
-// The products of a 64-column tile, issued by a whole warp for its elected lane. B operands are stages of 64 rows: D / 64 pieces of 64 x 128 bytes.
-template <int D, bool BF16>
-struct Products {
-    static constexpr uint32_t kHi = ptx::smem_desc_sw128_hi(1024);
-    static constexpr uint32_t kPiece = kHalf * 128;
-    static constexpr uint32_t kScores = ptx::mma_idesc_f16(BF16, false, false, kTile, kHalf);
-    static constexpr uint32_t kGrads = ptx::mma_idesc_f16(BF16, false, true, kTile, D);
-    // scores: rows of A (tensor memory) times the stage's rows, contraction over the head dim
-    static __device__ __forceinline__ void scores_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t stage) {
-        const uint32_t lo = ptx::smem_desc_sw128_lo(stage, 16);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) ptx::mma_ts_lead(lead, d, a + kk * 8, lo + (((kk / 4) * kPiece + (kk % 4) * 32) >> 4), kHi, kScores, kk != 0);
-    }
-    // the same with A as 128 rows in shared memory
-    static __device__ __forceinline__ void scores_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t stage) {
-        const uint32_t lo_a = ptx::smem_desc_sw128_lo(a, 16), lo_b = ptx::smem_desc_sw128_lo(stage, 16);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-            ptx::mma_ss_lead(lead, d, lo_a + (((kk / 4) * (kTile * 128) + (kk % 4) * 32) >> 4), lo_b + (((kk / 4) * kPiece + (kk % 4) * 32) >> 4), kHi, kScores, kk != 0);
-    }
-    // gradients: A (tensor memory, 64 columns of values) times the stage, contraction over its rows
-    static __device__ __forceinline__ void grads(uint32_t lead, uint32_t d, uint32_t a, uint32_t stage, bool first) {
-        const uint32_t lo = ptx::smem_desc_sw128_lo(stage, kPiece);
-#pragma unroll
-        for (int kk = 0; kk < kHalf / 16; ++kk) ptx::mma_ts_lead(lead, d, a + kk * 8, lo + ((kk * 16 * 128) >> 4), kHi, kGrads, !first || kk != 0);
-    }
-};
 template <int D, bool BF16, bool BIAS>
 __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, int item) {
     const CUtensorMap &map_q = m.q, &map_k = m.k_tile, &map_v = m.v_tile, &map_do = m.d_o, &map_dk = m.dk, &map_dv = m.dv;

@@ -1,15 +1,20 @@
 // Attention over heads, forward, on the tensor cores: f16 / bf16, d = 64 or 128.
 //
-// One CTA per (query tile, head, batch entry), two CTAs resident per SM (256 tensor-memory columns each), so that one's
-// softmax overlaps the other's products:
-//   warp 0    TMA: the Q tile once, 128-key K and V tiles, each re-armed as soon as the product that read it is done
-//   warp 1    tcgen05.mma: S = Q K^T into tensor memory, O += P V with P read from tensor memory
-//   warps 2-9 softmax, two threads per query row (64 keys of each tile apiece), one pass with a running maximum and sum;
-//             the maximum is raised only when it grows by more than 2^8, so O is rescaled rarely
-// Added to what plain attention does: the log-sum-exp of every row; grouped heads and strides through 4-D tensor maps; a
-// key count per batch entry (V rows behind it are cleared in shared memory before the product reads them, scores are masked
-// by selection, so nothing there is ever used); causal masks from either end; the relative position bias, one number for
-// blocks far from the diagonal, else 95 looked-up values per warp.
+// A CTA owns 128 query rows of a head and walks the keys 64 at a time. Warp 0 loads (TMA: the Q tile, rings of 64-row K and V
+// stages), warp 1 issues the products (S = Q K^T into tensor memory, O += P V with P read from there), and two groups of four warps
+// take the 64-key tiles in turn, one thread per row: while one group takes exponentials the products of the other's tile run. The
+// groups share nothing until the end: each keeps its own running maximum, sum and output accumulator, as if the row's keys had been
+// split over two CTAs, and the two are joined in the epilogue. The maximum is raised only when it grows by more than 2^8, so O is
+// rescaled rarely. (Before, two threads of different warps shared a row of a 128-key tile and traded its maximum through shared memory,
+// with everything on one chain S -> maximum -> trade -> exponentials -> O: 2200 cycles per 128 x 128 tile with two CTAs on the SM.)
+//   d = 128   one CTA per SM; S has two buffers per group, so the next S is there when a tile is done (512 tensor-memory columns)
+//   d = 64    two CTAs per SM of 256 columns, one S buffer per group: the exponentials are the limit (512 cycles of the transcendental
+//             unit per 128 x 64 tile against 320 of products), and the other CTA fills the gaps
+//
+// Beyond plain attention: the log-sum-exp of every row; grouped heads and strides through 4-D tensor maps; a key count per
+// batch entry (V rows behind it are cleared in shared memory before the product reads them, scores are masked by selection, so nothing
+// there is ever used); causal masks from either end; the relative position bias, one number for blocks far from the diagonal, else 95
+// looked-up values per warp.
 //
 // When there are few rows (single tokens against a cache) two things change. The query heads of a key head share one tile:
 // rows are (head of the group, query), loaded by one TMA box over both dimensions, so the keys are read once per key
@@ -44,61 +49,38 @@ __device__ uint32_t g_fwd_status;
 
 template <int D>
 struct FwdSmem {
-    static constexpr int kOperand = kTile * D * 2;
-    static constexpr int kBarOffset = 3 * kOperand;
-    static constexpr int kXchgOffset = kBarOffset + 256;
-    static constexpr int kBiasOffset = kXchgOffset + 2048;
-    static constexpr int kNeeded = kBiasOffset + (int)sizeof(BiasShared) + 1024;
-    static constexpr int kTotal = kNeeded > 81920 ? kNeeded : 81920;        // never three CTAs (of 256 tensor-memory columns) on an SM
+    static constexpr int kStage = kHalf * D * 2;
+    static constexpr int kStagesK = 4, kStagesV = 6;                    // V is held from its load to the end of the softmax
+    static constexpr int kBarOffset = (2 + kStagesK + kStagesV) * kStage;      // behind the Q tile and the rings
+    static constexpr int kMlOffset = kBarOffset + 512;                  // [2 groups][128] maximum and sum
+    static constexpr int kBiasOffset = kMlOffset + 2048;
+    static constexpr int kTotal = kBiasOffset + (int)sizeof(BiasShared) + 1024;
+    static_assert(D == 128 || (kTotal > 77824 && kTotal <= 115712), "two CTAs of 256 tensor-memory columns on an SM, never three");
 };
 
-// The two warps that share rows publish values in shared memory and trade a flag, with the time limit and abort handling of
-// every other wait. Returns false, warp-uniformly, when the wait was given up.
-__device__ __forceinline__ bool trade(const WaitCtx& ctx, volatile uint32_t* flags, int half, int quarter, int lane, uint32_t token, uint32_t code) {
-    __threadfence_block();
-    __syncwarp();
-    bool ok = true;
-    if (lane == 0) {
-        flags[half * 4 + quarter] = token;
-        volatile uint32_t* other = flags + (half ^ 1) * 4 + quarter;
-        uint64_t t0 = 0;
-        for (uint32_t spin = 1; *other != token; ++spin) {
-            if ((spin & 255u) == 0) {
-                if (*ctx.abort_flag) { ok = false; break; }
-                const uint64_t now = ptx::global_timer_ns();
-                if (t0 == 0) t0 = now;
-                else if (now - t0 > ctx.limit_ns) {
-                    atomicCAS(ctx.status_word, 0u, code);
-                    *ctx.abort_flag = 1;
-                    ok = false;
-                    break;
-                }
-            }
-        }
-    }
-    ok = __all_sync(0xffffffffu, ok);
-    __threadfence_block();
-    return ok;
-}
-
 template <int D, bool BF16, bool BIAS>
-__global__ void __launch_bounds__(kFwdThreads, 2)
+__global__ void __launch_bounds__(kFwdThreads, D == 64 ? 2 : 1)
 heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ CUtensorMap map_o, const __grid_constant__ FwdParams p) {
     using S = FwdSmem<D>;
-    constexpr int kChunks = D / 64;
-    constexpr uint32_t kTmemCols = 256, kColO = 128;
+    using Mma = Products<D, BF16>;
+    constexpr int kChunks = D / 64, kStagesK = S::kStagesK, kStagesV = S::kStagesV;
+    constexpr int kBuffers = D == 128 ? 4 : 2;                          // of S: tile h uses buffer h mod kBuffers
+    constexpr uint32_t kColO = 64 * kBuffers, kTmemCols = D == 128 ? 512 : 256;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
-    const uint32_t q_smem = smem_base, k_smem = smem_base + S::kOperand, v_smem = k_smem + S::kOperand;
+    const uint32_t q_smem = smem_base;
+    auto k_smem = [&](int s) { return smem_base + (2 + s) * S::kStage; };
+    auto v_smem = [&](int s) { return smem_base + (2 + kStagesK + s) * S::kStage; };
     const uint32_t bar_base = smem_base + S::kBarOffset;
-    const uint32_t q_full = bar_base, k_full = bar_base + 8, v_full = bar_base + 16, k_empty = bar_base + 24, v_empty = bar_base + 32,
-                   s_full = bar_base + 40, p_full = bar_base + 48, o_full = bar_base + 56, o_staged = bar_base + 64;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 80);
+    const uint32_t q_full = bar_base, acc_full = bar_base + 8, ml_ready = bar_base + 16, staged = bar_base + 24, s_full = bar_base + 32 /* per buffer */,
+                   p_ready = bar_base + 64 /* per buffer: a group may be two tiles ahead of the issuer */, o_done = bar_base + 96 /* per group */,
+                   k_full = bar_base + 128, k_empty = k_full + 8 * kStagesK,
+                   v_full = k_empty + 8 * kStagesK, v_empty = v_full + 8 * kStagesV;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + S::kBarOffset + 112);
     volatile uint32_t* abort_flag = tmem_slot + 1;
-    volatile uint32_t* pair_flags = tmem_slot + 4;                                  // [2 buffers][2 halves][4 quarters]
-    float* xchg = reinterpret_cast<float*>(smem_gen + S::kXchgOffset);              // [2][2][128]
+    float2* ml = reinterpret_cast<float2*>(smem_gen + S::kMlOffset);
     BiasShared& bias = *reinterpret_cast<BiasShared*>(smem_gen + S::kBiasOffset);
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -113,37 +95,40 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const int n_keys = heads_key_count(p.h, b), offset = heads_offset(p.h, n_keys);
     const int last_query = p.packed ? p.h.seq_q - 1 : min(row0 + kTile, p.h.seq_q) - 1;
     const int key_end = p.h.causal ? max(0, min(n_keys, last_query + offset + 1)) : n_keys;
-    const int all_tiles = (key_end + kTile - 1) / kTile;
-    const int tile_first = (int)((long long)all_tiles * split / p.splits);
-    const int kv_tiles = (int)((long long)all_tiles * (split + 1) / p.splits) - tile_first;
+    const int all_tiles = (key_end + kHalf - 1) / kHalf;
+    int first = 0, n_it = all_tiles;                                    // this CTA's tiles
+    if (p.splits > 1) {
+        first = (int)((long long)all_tiles * split / p.splits);
+        n_it = (int)((long long)all_tiles * (split + 1) / p.splits) - first;
+    }
     const WaitCtx wctx{abort_flag, p.status, p.wait_limit_ns};
 
-    auto load_k = [&](int j) {
-        ptx::mbar_arrive_expect_tx(k_full, S::kOperand);
+    auto load_k = [&](int s, int it) {
+        ptx::mbar_arrive_expect_tx(k_full + 8 * s, S::kStage);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
-            ptx::tma_load_4d(k_smem + c * (kTile * 128), &map_k, k_full, c * 64, (tile_first + j) * kTile, hk * p.k_at.head, b * p.k_at.batch);
+            ptx::tma_load_4d(k_smem(s) + c * Mma::kPiece, &map_k, k_full + 8 * s, c * 64, (first + it) * kHalf, hk * p.k_at.head, b * p.k_at.batch);
     };
-    auto load_v = [&](int j) {
-        ptx::mbar_arrive_expect_tx(v_full, S::kOperand);
+    auto load_v = [&](int s, int it) {
+        ptx::mbar_arrive_expect_tx(v_full + 8 * s, S::kStage);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
-            ptx::tma_load_4d(v_smem + c * (kTile * 128), &map_v, v_full, c * 64, (tile_first + j) * kTile, hk * p.v_at.head, b * p.v_at.batch);
+            ptx::tma_load_4d(v_smem(s) + c * Mma::kPiece, &map_v, v_full + 8 * s, c * 64, (first + it) * kHalf, hk * p.v_at.head, b * p.v_at.batch);
     };
     if (threadIdx.x == 0) {
-        ptx::mbar_init(q_full, 1); ptx::mbar_init(k_full, 1); ptx::mbar_init(v_full, 1);
-        ptx::mbar_init(k_empty, 1); ptx::mbar_init(v_empty, 1);
-        ptx::mbar_init(s_full, 1); ptx::mbar_init(p_full, 8); ptx::mbar_init(o_full, 1); ptx::mbar_init(o_staged, 8);
-        for (int q = 0; q < 16; ++q) pair_flags[q] = 0;
+        ptx::mbar_init(q_full, 1); ptx::mbar_init(acc_full, 1); ptx::mbar_init(ml_ready, 8); ptx::mbar_init(staged, 8);
+        for (int y = 0; y < kBuffers; ++y) { ptx::mbar_init(s_full + 8 * y, 1); ptx::mbar_init(p_ready + 8 * y, 4); }
+        ptx::mbar_init(o_done, 1); ptx::mbar_init(o_done + 8, 1);
+        for (int s = 0; s < kStagesK; ++s) { ptx::mbar_init(k_full + 8 * s, 1); ptx::mbar_init(k_empty + 8 * s, 1); }
+        for (int s = 0; s < kStagesV; ++s) { ptx::mbar_init(v_full + 8 * s, 1); ptx::mbar_init(v_empty + 8 * s, 1); }
         *abort_flag = 0;
         ptx::mbar_fence_init();
-        if (kv_tiles > 0) {                                     // the first loads fly while the CTA sets itself up
+        if (n_it > 0) {                                                 // the first loads fly while the CTA sets itself up
             ptx::mbar_arrive_expect_tx(q_full, box_rows * D * 2);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c)
                 ptx::tma_load_4d(q_smem + c * (kTile * 128), &map_q, q_full, c * 64, row0, head0 * p.q_at.head, b * p.q_at.batch);
-            load_k(0);
-            load_v(0);
+            load_k(0, 0);
         }
     }
     if constexpr (BIAS) {
@@ -164,208 +149,215 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (warp == 0) {
         // ---- TMA producer ------------------------------------------------------------------------------
         if (lane == 0) {
-            for (int j = 1; j < kv_tiles; ++j) {
-                if (!bounded_wait(wctx, k_empty, (j & 1) ^ 1, 0x04010000u | (j & 0xffff))) break;
-                load_k(j);
-                if (!bounded_wait(wctx, v_empty, (j & 1) ^ 1, 0x04020000u | (j & 0xffff))) break;
-                load_v(j);
+            int ks = 0, vs = 0;
+            uint32_t k_phase = 1, v_phase = 1;
+            for (int it = 0; it < n_it; ++it) {
+                if (it > 0) {
+                    if (!bounded_wait(wctx, k_empty + 8 * ks, k_phase, 0x04010000u | (it & 0xffff))) break;
+                    load_k(ks, it);
+                }
+                if (!bounded_wait(wctx, v_empty + 8 * vs, v_phase, 0x04020000u | (it & 0xffff))) break;
+                load_v(vs, it);
+                if (++ks == kStagesK) { ks = 0; k_phase ^= 1; }
+                if (++vs == kStagesV) { vs = 0; v_phase ^= 1; }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        // ---- MMA issuer: the whole warp, for its elected lane -----------------------------------------------
+        // ---- MMA issuer, the whole warp for its elected lane: S(0) .. | O += P(i) V(i), S(i + kBuffers) | ... -----------
         {
-            constexpr uint32_t idesc_s = ptx::mma_idesc_f16(BF16, false, false, kTile, kTile);
-            constexpr uint32_t idesc_o = ptx::mma_idesc_f16(BF16, false, true, kTile, D);
-            constexpr uint32_t hi = ptx::smem_desc_sw128_hi(1024);
             const uint32_t lead = ptx::elect_lead();
-            const uint32_t q_lo = ptx::smem_desc_sw128_lo(q_smem, 16), k_lo = ptx::smem_desc_sw128_lo(k_smem, 16), v_lo = ptx::smem_desc_sw128_lo(v_smem, kTile * 128);
             const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
-            const int tiles = __shfl_sync(0xffffffffu, kv_tiles, 0);
-            auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) { return warp_spin(wctx, bar, parity, code); };
-            const uint32_t s_tmem = tmem, o_tmem = tmem + kColO;
-            bool ok = tiles == 0 || wait(q_full, 0, 0x04030000u);
-            for (int j = 0; j < tiles && ok; ++j) {
-                const uint32_t ph = j & 1;
-                if (!(ok = wait(k_full, ph, 0x04040000u | (j & 0xffff)))) break;
+            const int tiles = __shfl_sync(0xffffffffu, n_it, 0);
+            int ks = 0, vs = 0;
+            uint32_t k_phase = 0, v_phase = 0;
+            auto s_product = [&](int it) {
+                if (!warp_spin(wctx, k_full + 8 * ks, k_phase, 0x04030000u | (it & 0xffff))) return false;
                 ptx::tc_fence_after_sync();
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {           // S = Q K^T, contraction over the head dim
-                    const uint32_t off = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) >> 4;
-                    ptx::mma_ss_lead(lead, s_tmem, q_lo + off, k_lo + off, hi, idesc_s, kk != 0);
-                }
-                ptx::mma_commit_lead(lead, s_full);
-                ptx::mma_commit_lead(lead, k_empty);
-                if (!(ok = wait(p_full, ph, 0x04050000u | (j & 0xffff)))) break;
-                if (!(ok = wait(v_full, ph, 0x04060000u | (j & 0xffff)))) break;
+                Mma::scores_ss(lead, tmem + 64 * (it % kBuffers), q_smem, k_smem(ks));
+                ptx::mma_commit_lead(lead, s_full + 8 * (it % kBuffers));
+                ptx::mma_commit_lead(lead, k_empty + 8 * ks);
+                if (++ks == kStagesK) { ks = 0; k_phase ^= 1; }
+                return true;
+            };
+            bool ok = tiles == 0 || warp_spin(wctx, q_full, 0, 0x04040000u);
+            for (int it = 0; it < kBuffers && it < tiles && ok; ++it) ok = s_product(it);
+            for (int it = 0; it < tiles && ok; ++it) {
+                if (!(ok = warp_spin(wctx, v_full + 8 * vs, v_phase, 0x04050000u | (it & 0xffff)))) break;
+                if (!(ok = warp_spin(wctx, p_ready + 8 * (it % kBuffers), (it / kBuffers) & 1, 0x04060000u | (it & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
-#pragma unroll
-                for (int kk = 0; kk < kTile / 16; ++kk)         // O += P V, contraction over the keys
-                    ptx::mma_ts_lead(lead, o_tmem, s_tmem + kk * 8, v_lo + ((kk * 16 * 128) >> 4), hi, idesc_o, (j | kk) != 0);
-                ptx::mma_commit_lead(lead, v_empty);
+                Mma::grads(lead, tmem + kColO + D * (it & 1), tmem + 64 * (it % kBuffers), v_smem(vs), it < 2);
+                ptx::mma_commit_lead(lead, o_done + 8 * (it & 1));
+                ptx::mma_commit_lead(lead, v_empty + 8 * vs);
+                if (it + kBuffers < tiles && !(ok = s_product(it + kBuffers))) break;
+                if (++vs == kStagesV) { vs = 0; v_phase ^= 1; }
             }
-            if (ok) ptx::mma_commit_lead(lead, o_full);
+            if (ok) ptx::mma_commit_lead(lead, acc_full);
         }
         __syncwarp();
     } else {
-        // ---- softmax: two threads per query row, 64 keys of each tile apiece ----------------------------------
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        // ---- softmax: one thread per query row; group x takes tiles x, x + 2, ... -----------------------------------------
+        const int w = warp - 2, quarter = warp & 3, x = w >> 2;
         const int row_in_tile = quarter * 32 + lane;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        const uint32_t s_row = tmem_base + lane_base + half * (kTile / 2);
-        const uint32_t p_row = tmem_base + lane_base + half * (kTile / 4);
-        const uint32_t o_row = tmem_base + lane_base + kColO + half * (D / 2);
+        const uint32_t o_row = tmem_base + lane_base + kColO + x * D;
         const int query = p.packed ? row_in_tile % p.h.seq_q : row0 + row_in_tile;
-        // keys 0 .. sees - 1 are seen by this row
-        const int sees = p.h.causal ? min(n_keys, query + offset + 1) : n_keys;
+        const int sees = p.h.causal ? min(n_keys, query + offset + 1) : n_keys;         // keys 0 .. sees - 1
         float m_run = -CUDART_INF_F;      // the max the exponentials are taken against (log2 units)
-        float l_run = 0.0f;               // running sum over this thread's columns
+        float l_run = 0.0f;
         bool ok = true;
         WarpBias wb(p.h);
-        for (int j = 0; j < kv_tiles && ok; ++j) {
-            const int key0 = (tile_first + j) * kTile + half * (kTile / 2);
+        for (int it = x; it < n_it && ok; it += 2) {
+            const int key0 = (first + it) * kHalf;
+            const uint32_t s_at = tmem_base + lane_base + 64 * (it % kBuffers);
             float c = p.h.scale_log2, add = 0.0f;               // a score in log2 units is c * s + add
             bool looked_up = false;
-            if constexpr (BIAS) looked_up = !wb.block(bias, bias.value, warp - 2, lane, p.h.n_runs, key0 - (row0 + quarter * 32 + 31 + offset));
-            ok = __all_sync(0xffffffffu, bounded_wait(wctx, s_full, j & 1, 0x04070000u | (j & 0xffff)));
+            if constexpr (BIAS) looked_up = !wb.block(bias, bias.value, w, lane, p.h.n_runs, key0 - (row0 + quarter * 32 + 31 + offset));
+            ok = warp_wait(wctx, s_full + 8 * (it % kBuffers), (it / kBuffers) & 1, 0x04070000u | (it & 0xffff));
             if (!ok) break;
             ptx::tc_fence_after_sync();
-            uint32_t r[kTile / 2];
-#pragma unroll
-            for (int ch = 0; ch < kTile / 64; ++ch) ptx::tmem_ld_32x32b_x32(s_row + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[ch * 32]));
+            uint32_t r[64];
+            ptx::tmem_ld_32x32b_x32(s_at, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+            ptx::tmem_ld_32x32b_x32(s_at + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
             ptx::tmem_ld_wait();
             if constexpr (BIAS) {
                 if (looked_up) {
-                    const float* at = bias.by_dist[warp - 2] + 31 - lane;
+                    const float* at = bias.by_dist[w] + 31 - lane;
 #pragma unroll
-                    for (int i = 0; i < kTile / 2; ++i) r[i] = __float_as_uint(fmaf(__uint_as_float(r[i]), c, at[i]));
+                    for (int i = 0; i < 64; ++i) r[i] = __float_as_uint(fmaf(__uint_as_float(r[i]), c, at[i]));
                     c = 1.0f;
                 } else {
                     add = wb.same;
                 }
             }
-            const int valid = sees - key0;                      // of this thread's columns
-            if (valid < kTile / 2) {
+            const int valid = sees - key0;                      // columns that are seen
+            if (valid < 64) {
 #pragma unroll
-                for (int i = 0; i < kTile / 2; ++i)
+                for (int i = 0; i < 64; ++i)
                     if (i >= valid) r[i] = __float_as_uint(-CUDART_INF_F);
             }
             float ext[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) ext[i] = __uint_as_float(r[i]);
 #pragma unroll
-            for (int i = 8; i < kTile / 2; ++i) ext[i & 7] = fmaxf(ext[i & 7], __uint_as_float(r[i]));
+            for (int i = 8; i < 64; ++i) ext[i & 7] = fmaxf(ext[i & 7], __uint_as_float(r[i]));
             ext[0] = fmaxf(fmaxf(fmaxf(ext[0], ext[1]), fmaxf(ext[2], ext[3])), fmaxf(fmaxf(ext[4], ext[5]), fmaxf(ext[6], ext[7])));
-            const float mine = fmaf(ext[0], c, add);
-            // exchange with the thread that owns the other half of the row (after it both halves of S are in registers, so P may
-            // overwrite S)
-            volatile float* slot = xchg + (j & 1) * 256;
-            slot[half * 128 + row_in_tile] = mine;
-            ok = trade(wctx, pair_flags + (j & 1) * 8, half, quarter, lane, (uint32_t)j + 1, 0x04090000u | (j & 0xffff));
-            if (!ok) break;
-            const float m_tile = fmaxf(mine, slot[(half ^ 1) * 128 + row_in_tile]);
+            const float m_tile = fmaf(ext[0], c, add);
             const bool raise = m_tile > m_run + 8.0f;           // from -inf: with the first key the row sees
-            const float m_new = raise ? m_tile : m_run;
-            if (__any_sync(0xffffffffu, raise) && j > 0) {
-                const float f = raise ? ptx::ex2_approx(m_run - m_new) : 1.0f;
+            if (__any_sync(0xffffffffu, raise)) {
+                const float f = raise ? ptx::ex2_approx(m_run - m_tile) : 1.0f;
+                if (it >= 2) {                                  // O holds the group's earlier tiles, once the last of them has been added
+                    ok = warp_wait(wctx, o_done + 8 * x, ((it - 2) >> 1) & 1, 0x04080000u | (it & 0xffff));
+                    if (!ok) break;
+                    ptx::tc_fence_after_sync();
 #pragma unroll 1
-                for (int col = 0; col < D / 2; col += 8) {      // few registers: the S row is still live
-                    uint32_t o[8];
-                    ptx::tmem_ld_32x32b_x8(o_row + col, o);
-                    ptx::tmem_ld_wait();
+                    for (int col = 0; col < D; col += 8) {      // few registers: the S row is still live
+                        uint32_t o[8];
+                        ptx::tmem_ld_32x32b_x8(o_row + col, o);
+                        ptx::tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                    ptx::tmem_st_32x32b_x8(o_row + col, o);
+                        for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        ptx::tmem_st_32x32b_x8(o_row + col, o);
+                    }
                 }
                 l_run *= f;
+                if (raise) m_run = m_tile;
             }
-            m_run = m_new;
             const float ref = m_run == -CUDART_INF_F ? 0.0f : m_run;            // nothing seen so far: every exponential is 2^-inf
             const float shift = add - ref + (BF16 ? kCutScaleLog2 : 0.0f);
             const float2 c2 = make_float2(c, c), s2 = make_float2(shift, shift);
             float2 sum2[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-            for (int ch = 0; ch < kTile / 64; ++ch) {
-                uint32_t w[16];
+            for (int ch = 0; ch < 2; ++ch) {
+                uint32_t pk[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float2 y = fma2(f2(r[ch * 32 + 2 * i], r[ch * 32 + 2 * i + 1]), c2, s2);
                     const float2 e = make_float2(ptx::ex2_approx(y.x), ptx::ex2_approx(y.y));
                     sum2[i & 3] = add2(sum2[i & 3], e);
-                    w[i] = operand_pair<BF16>(e);
+                    pk[i] = operand_pair<BF16>(e);
                 }
-                ptx::tmem_st_32x32b_x16(p_row + ch * 16, w);
+                ptx::tmem_st_32x32b_x16(s_at + ch * 16, pk);
             }
             const float2 tot = add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3]));
             l_run += tot.x + tot.y;
             // V rows behind the key count hold whatever the caller left there: cleared before the product multiplies them by P's zeros
-            const int live = n_keys - (tile_first + j) * kTile;
-            if (live < kTile && n_keys < p.h.seq_k) {
-                ok = __all_sync(0xffffffffu, bounded_wait(wctx, v_full, j & 1, 0x040b0000u | (j & 0xffff)));
+            const int live = n_keys - key0;
+            if (live < kHalf && n_keys < p.h.seq_k) {
+                const int vs = it % kStagesV;
+                ok = warp_wait(wctx, v_full + 8 * vs, (it / kStagesV) & 1, 0x04090000u | (it & 0xffff));
                 if (!ok) break;
-                for (int e = live * 8 + (int)threadIdx.x - 64; e < kTile * 8; e += 256)         // 16-byte pieces of the rows
+                for (int e = live * 8 + row_in_tile; e < kHalf * 8; e += 128)           // 16-byte pieces of the rows
 #pragma unroll
                     for (int ch = 0; ch < kChunks; ++ch)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_smem + ch * (kTile * 128) + e * 16), "r"(0) : "memory");
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_smem(vs) + ch * Mma::kPiece + e * 16), "r"(0) : "memory");
                 ptx::fence_proxy_async_smem();
             }
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(p_full);
+            if (lane == 0) ptx::mbar_arrive(p_ready + 8 * (it % kBuffers));
         }
-        // merge the two partial row sums, then write this thread's half of the output row
+        // ---- the two groups joined; each writes half of the columns ----------------------------------------------------------
         if (ok) {
-            volatile float* slot = xchg + (kv_tiles & 1) * 256;
-            slot[half * 128 + row_in_tile] = l_run;
-            ok = trade(wctx, pair_flags + (kv_tiles & 1) * 8, half, quarter, lane, (uint32_t)kv_tiles + 1, 0x040a0000u);
-            if (ok) l_run += slot[(half ^ 1) * 128 + row_in_tile];
+            ml[x * 128 + row_in_tile] = make_float2(m_run, l_run);
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ml_ready);
+            ok = warp_wait(wctx, ml_ready, 0, 0x040a0000u) && warp_wait(wctx, acc_full, 0, 0x040b0000u);
         }
-        if (ok && __all_sync(0xffffffffu, bounded_wait(wctx, o_full, 0, 0x04080000u))) {
+        if (ok) {
             ptx::tc_fence_after_sync();
+            const float2 a = ml[row_in_tile], z = ml[128 + row_in_tile];
+            const bool has_a = a.y != 0.0f, has_z = z.y != 0.0f;        // otherwise the group saw no key of the row
+            const float m = fmaxf(has_a ? a.x : -CUDART_INF_F, has_z ? z.x : -CUDART_INF_F), ref = m == -CUDART_INF_F ? 0.0f : m;
+            const float fa = has_a ? ptx::ex2_approx(a.x - ref) : 0.0f, fz = has_z ? ptx::ex2_approx(z.x - ref) : 0.0f;
+            const float l = (has_a ? a.y * fa : 0.0f) + (has_z ? z.y * fz : 0.0f);
+            const bool empty = !has_a && !has_z;
             const bool live_row = p.packed ? row_in_tile < box_rows : query < p.h.seq_q;
             const int head = p.packed ? head0 + row_in_tile / p.h.seq_q : head0;
-            const int64_t out_row = ((int64_t)b * p.h.heads + head) * p.h.seq_q + query;
-            const bool empty = l_run == 0.0f;                   // the row saw no key
-            if (p.splits > 1) {
-                const int64_t at = (int64_t)split * p.h.batch * p.h.heads * p.h.seq_q + out_row;
+            const int64_t rows = (int64_t)p.h.batch * p.h.heads * p.h.seq_q, out_row = ((int64_t)b * p.h.heads + head) * p.h.seq_q + query;
+            const bool parts = p.splits > 1;
+            const float inv = parts ? 1.0f : empty ? 0.0f : (BF16 ? kCutScale : 1.0f) / l;
+            const float2 wa = make_float2(fa * inv, fa * inv), wz = make_float2(fz * inv, fz * inv);
 #pragma unroll 1
-                for (int ch = 0; ch < D / 16; ++ch) {           // this thread's D / 2 columns, eight at a time
-                    uint32_t o[8];
-                    ptx::tmem_ld_32x32b_x8(o_row + ch * 8, o);
-                    ptx::tmem_ld_wait();
-                    if (live_row && !empty) {
-                        float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + half * (D / 2) + ch * 8);
-                        dst[0] = make_float4(__uint_as_float(o[0]), __uint_as_float(o[1]), __uint_as_float(o[2]), __uint_as_float(o[3]));
-                        dst[1] = make_float4(__uint_as_float(o[4]), __uint_as_float(o[5]), __uint_as_float(o[6]), __uint_as_float(o[7]));
-                    }
-                }
-                if (live_row && half == 0) p.part_ml[at] = make_float2(m_run, l_run);
-            } else {
-                if (live_row && half == 0)
-                    p.lse[out_row] = empty ? -CUDART_INF_F : (m_run + log2f(l_run) - (BF16 ? kCutScaleLog2 : 0.0f)) * kLn2;
-                // every product has completed, so the Q tile's shared memory is free: the output is staged there and leaves through TMA
-                const float inv = empty ? 0.0f : (BF16 ? kCutScale : 1.0f) / l_run;
-#pragma unroll 1
-                for (int ch = 0; ch < D / 64; ++ch) {
-                    uint32_t o[32];
-                    ptx::tmem_ld_32x32b_x32(o_row + ch * 32, o);
-                    ptx::tmem_ld_wait();
-                    uint32_t w[16];
+            for (int ch = 0; ch < D / 64; ++ch) {               // this group's D / 2 columns, 32 at a time
+                const int col = x * (D / 2) + ch * 32;
+                uint32_t oa[32], oz[32];
+                ptx::tmem_ld_32x32b_x32(tmem_base + lane_base + kColO + col, oa);
+                ptx::tmem_ld_32x32b_x32(tmem_base + lane_base + kColO + D + col, oz);
+                ptx::tmem_ld_wait();
+                float2 o[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        w[i] = empty ? 0u : round_pair<BF16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-                    stage_row(q_smem, row_in_tile, half * (D / 2) + ch * 32, w);
+                for (int i = 0; i < 16; ++i) {                  // what a group without keys left in its accumulator is not looked at
+                    const float2 va = has_a ? mul2(f2(oa[2 * i], oa[2 * i + 1]), wa) : make_float2(0.0f, 0.0f);
+                    o[i] = has_z ? fma2(f2(oz[2 * i], oz[2 * i + 1]), wz, va) : va;
                 }
+                if (parts) {
+                    if (live_row && !empty) {
+                        float4* dst = reinterpret_cast<float4*>(p.part_o + (split * rows + out_row) * D + col);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[2 * i].x, o[2 * i].y, o[2 * i + 1].x, o[2 * i + 1].y);
+                    }
+                } else {                                        // every product has completed: the output is staged over Q and leaves through TMA
+                    uint32_t v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = round_pair<BF16>(o[i].x, o[i].y);
+                    stage_row(q_smem, row_in_tile, col, v);
+                }
+            }
+            if (parts) {
+                if (live_row && x == 0) p.part_ml[split * rows + out_row] = make_float2(m, empty ? 0.0f : l);
+            } else {
+                if (live_row && x == 0) p.lse[out_row] = empty ? -CUDART_INF_F : (m + log2f(l) - (BF16 ? kCutScaleLog2 : 0.0f)) * kLn2;
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(o_staged);
-                if (threadIdx.x == 64 && bounded_wait(wctx, o_staged, 0, 0x040c0000u)) {
+                if (lane == 0) ptx::mbar_arrive(staged);
+                if (w == 0 && lane == 0 && bounded_wait(wctx, staged, 0, 0x040c0000u)) {
 #pragma unroll
-                    for (int c = 0; c < kChunks; ++c)
-                        ptx::tma_store_4d(&map_o, q_smem + c * (kTile * 128), c * 64, row0, head0 * p.o_at.head, b * p.o_at.batch);
+                    for (int ch = 0; ch < kChunks; ++ch)        // rows that do not exist are dropped
+                        ptx::tma_store_4d(&map_o, q_smem + ch * (kTile * 128), ch * 64, row0, head0 * p.o_at.head, b * p.o_at.batch);
                     ptx::tma_store_commit();
-                    ptx::tma_store_wait_read<0>();     // shared memory has been read; the grid's end covers the writes
+                    ptx::tma_store_wait_read<0>();              // shared memory has been read; the grid's end covers the writes
                 }
             }
         }
@@ -427,8 +419,8 @@ static int launch(FwdParams& p, const FwdPlan& plan, const void* Q, const void* 
     CUtensorMap mq, mk, mv, mo;
     const int q_rows = plan.packed ? p.h.seq_q : kTile, q_heads = plan.packed ? p.h.group : 1;
     int rc = make_map(&mq, &p.q_at, Q, p.h.batch, p.h.heads, p.h.seq_q, D, p.h.q_s, q_rows, q_heads);
-    if (rc == EMMYB200_OK) rc = make_map(&mk, &p.k_at, K, p.h.batch, p.h.kv_heads, p.h.seq_k, D, p.h.k_s, kTile, 1);
-    if (rc == EMMYB200_OK) rc = make_map(&mv, &p.v_at, V, p.h.batch, p.h.kv_heads, p.h.seq_k, D, p.h.v_s, kTile, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&mk, &p.k_at, K, p.h.batch, p.h.kv_heads, p.h.seq_k, D, p.h.k_s, kHalf, 1);
+    if (rc == EMMYB200_OK) rc = make_map(&mv, &p.v_at, V, p.h.batch, p.h.kv_heads, p.h.seq_k, D, p.h.v_s, kHalf, 1);
     if (rc == EMMYB200_OK) rc = make_map(&mo, &p.o_at, O, p.h.batch, p.h.heads, p.h.seq_q, D, p.h.o_s, q_rows, q_heads);
     if (rc != EMMYB200_OK) return rc;
     EMMY_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p.status), g_fwd_status));

@@ -11,7 +11,8 @@
 namespace emmy {
 namespace heads {
 
-constexpr int kTile = 128;              // query rows and keys of a tile
+constexpr int kTile = 128;              // rows of a tile: tensor-memory lanes
+constexpr int kHalf = 64;               // columns of a tile: rows of a stage
 // bf16 operands of second products are cut from the fp32 pattern (one byte permute per pair): a conversion would run on the
 // transcendental unit next to the exponentials. A cut loses half a step, 2^-8 of a value with mantissa 1, on average 2^-8 / ln 4 of
 // values spread evenly in magnitude: they are scaled by 1 + 2^-8 / ln 4 first, which leaves no mean error and at most 1.28 times the
@@ -154,6 +155,33 @@ struct WarpBias {
     }
 };
 
+// The products of a 64-column tile, issued by a whole warp for its elected lane. B operands are stages of 64 rows: D / 64 pieces of 64 x 128 bytes.
+template <int D, bool BF16>
+struct Products {
+    static constexpr uint32_t kHi = ptx::smem_desc_sw128_hi(1024);
+    static constexpr uint32_t kPiece = kHalf * 128;
+    static constexpr uint32_t kScores = ptx::mma_idesc_f16(BF16, false, false, kTile, kHalf);
+    static constexpr uint32_t kGrads = ptx::mma_idesc_f16(BF16, false, true, kTile, D);
+    // scores: rows of A (tensor memory) times the stage's rows, contraction over the head dim
+    static __device__ __forceinline__ void scores_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t stage) {
+        const uint32_t lo = ptx::smem_desc_sw128_lo(stage, 16);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) ptx::mma_ts_lead(lead, d, a + kk * 8, lo + (((kk / 4) * kPiece + (kk % 4) * 32) >> 4), kHi, kScores, kk != 0);
+    }
+    // the same with A as 128 rows in shared memory
+    static __device__ __forceinline__ void scores_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t stage) {
+        const uint32_t lo_a = ptx::smem_desc_sw128_lo(a, 16), lo_b = ptx::smem_desc_sw128_lo(stage, 16);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+            ptx::mma_ss_lead(lead, d, lo_a + (((kk / 4) * (kTile * 128) + (kk % 4) * 32) >> 4), lo_b + (((kk / 4) * kPiece + (kk % 4) * 32) >> 4), kHi, kScores, kk != 0);
+    }
+    // gradients: A (tensor memory, 64 columns of values) times the stage, contraction over its rows
+    static __device__ __forceinline__ void grads(uint32_t lead, uint32_t d, uint32_t a, uint32_t stage, bool first) {
+        const uint32_t lo = ptx::smem_desc_sw128_lo(stage, kPiece);
+#pragma unroll
+        for (int kk = 0; kk < kHalf / 16; ++kk) ptx::mma_ts_lead(lead, d, a + kk * 8, lo + ((kk * 16 * 128) >> 4), kHi, kGrads, !first || kk != 0);
+    }
+};
 // ---- the order of the work items -----------------------------------------------------------------------------------------------
 // Causal tiles differ in length. Dealt longest first over many units the SMs finish together; dealt unit by unit the last units'
 // longest tiles run alone (16 units of 2048 keys on 148 SMs: 184 us against 118). But CTAs that run at the same time should share
