@@ -72,22 +72,6 @@ __device__ __forceinline__ float ds_scale(float do_norm, float v_norm) {
     return __int_as_float(((int)fminf(fmaxf(floorf(-log2f(bound)), -100.0f), 100.0f) + 127) << 23);
 }
 
-// A row of a 128-row tile in shared memory (pieces of 128 rows x 64 elements, 128-byte swizzle) into tensor memory, as the A operand of a
-// product: D / 2 columns of element pairs. (Threads reading their rows from global memory instead took 7000 cycles of a CTA's set-up.)
-template <int D>
-__device__ __forceinline__ void row_to_tmem(uint32_t taddr, uint32_t tile, int row) {
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {          // 32 elements
-        uint32_t r[16];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int piece = (i % 2) * 4 + k;
-            ptx::ld_shared_16B(tile + (i / 2) * (kTile * 128) + row * 128 + ((piece ^ (row & 7)) << 4), r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
-        }
-        ptx::tmem_st_32x32b_x16(taddr + 16 * i, r);
-    }
-}
-
 template <int D, bool BF16, bool BIAS>
 __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, int item) {
     const CUtensorMap &map_q = m.q, &map_k = m.k_tile, &map_v = m.v_tile, &map_do = m.d_o, &map_dk = m.dk, &map_dv = m.dv;
@@ -240,7 +224,7 @@ __device__ __forceinline__ void dkv_block(const BwdMaps& m, const BwdParams& p, 
         const uint32_t s_at = tmem_base + lane_base + kColS + x * 64, dp_at = tmem_base + lane_base + kColDP + x * 64;
         bool ok = true;
         if (kKvInTmem && n_it > 0 && (ok = warp_wait(wctx, kv_full, 0, 0x05090000u))) {          // group 0 writes K to tensor memory, group 1 V
-            row_to_tmem<D>(tmem_base + lane_base + (x ? kColV : kColK), x ? v_smem : k_smem, quarter * 32 + lane);
+            row_to_tmem<D / 32>(tmem_base + lane_base + (x ? kColV : kColK), x ? v_smem : k_smem, quarter * 32 + lane);
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
             __syncwarp();
@@ -572,7 +556,7 @@ __device__ __forceinline__ void dq_block(const BwdMaps& m, const BwdParams& p, i
         const uint32_t s_at = tmem_base + lane_base + kColS + x * 64, dp_at = tmem_base + lane_base + kColDP + x * 64;
         bool ok = true;
         if (n_it > 0 && (ok = warp_wait(wctx, a_full, 0, 0x06020000u))) {        // group 0 writes Q to tensor memory, group 1 dO
-            row_to_tmem<D>(tmem_base + lane_base + (x ? kColDO : kColQ), x ? v_smem(kStages - 2) : k_smem(kStages - 2), quarter * 32 + lane);
+            row_to_tmem<D / 32>(tmem_base + lane_base + (x ? kColDO : kColQ), x ? v_smem(kStages - 2) : k_smem(kStages - 2), quarter * 32 + lane);
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
             __syncwarp();

@@ -1,13 +1,15 @@
 // Attention over heads, forward, on the tensor cores: f16 / bf16, d = 64 or 128.
 //
 // A CTA owns 128 query rows of a head and walks the keys 64 at a time. Warp 0 loads (TMA: the Q tile, rings of 64-row K and V
-// stages), warp 1 issues the products (S = Q K^T into tensor memory, O += P V with P read from there), and two groups of four warps
+// stages), warp 1 issues the products (S = Q K^T into tensor memory, O += P V with P read from there, over the S it came from), and two groups of four warps
 // take the 64-key tiles in turn, one thread per row: while one group takes exponentials the products of the other's tile run. The
 // groups share nothing until the end: each keeps its own running maximum, sum and output accumulator, as if the row's keys had been
 // split over two CTAs, and the two are joined in the epilogue. The maximum is raised only when it grows by more than 2^8, so O is
 // rescaled rarely. (Before, two threads of different warps shared a row of a 128-key tile and traded its maximum through shared memory,
 // with everything on one chain S -> maximum -> trade -> exponentials -> O: 2200 cycles per 128 x 128 tile with two CTAs on the SM.)
-//   d = 128   one CTA per SM; S has two buffers per group, so the next S is there when a tile is done (512 tensor-memory columns)
+//   d = 128   one CTA per SM; Q is written to tensor memory once and read from there (a product with N = 64 and both operands in
+//             shared memory takes 48 cycles per step instead of 32), and S has three buffers, so that a group's next S is there when its
+//             tile is done (512 columns: S 3 x 64, O 2 x 128, Q 64)
 //   d = 64    two CTAs per SM of 256 columns, one S buffer per group: the exponentials are the limit (512 cycles of the transcendental
 //             unit per 128 x 64 tile against 320 of products), and the other CTA fills the gaps
 //
@@ -65,8 +67,9 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     using S = FwdSmem<D>;
     using Mma = Products<D, BF16>;
     constexpr int kChunks = D / 64, kStagesK = S::kStagesK, kStagesV = S::kStagesV;
-    constexpr int kBuffers = D == 128 ? 4 : 2;                          // of S: tile h uses buffer h mod kBuffers
-    constexpr uint32_t kColO = 64 * kBuffers, kTmemCols = D == 128 ? 512 : 256;
+    constexpr bool kQInTmem = D == 128;
+    constexpr int kBuffers = D == 128 ? 3 : 2;                          // of S: tile h uses buffer h mod kBuffers
+    constexpr uint32_t kColO = 64 * kBuffers, kColQ = kColO + 2 * D, kTmemCols = D == 128 ? 512 : 256;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
@@ -74,7 +77,7 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     auto k_smem = [&](int s) { return smem_base + (2 + s) * S::kStage; };
     auto v_smem = [&](int s) { return smem_base + (2 + kStagesK + s) * S::kStage; };
     const uint32_t bar_base = smem_base + S::kBarOffset;
-    const uint32_t q_full = bar_base, acc_full = bar_base + 8, ml_ready = bar_base + 16, staged = bar_base + 24, s_full = bar_base + 32 /* per buffer */,
+    const uint32_t q_full = bar_base, q_ready = kQInTmem ? bar_base + 120 : q_full, acc_full = bar_base + 8, ml_ready = bar_base + 16, staged = bar_base + 24, s_full = bar_base + 32 /* per buffer */,
                    p_ready = bar_base + 64 /* per buffer: a group may be two tiles ahead of the issuer */, o_done = bar_base + 96 /* per group */,
                    k_full = bar_base + 128, k_empty = k_full + 8 * kStagesK,
                    v_full = k_empty + 8 * kStagesK, v_empty = v_full + 8 * kStagesV;
@@ -116,7 +119,8 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             ptx::tma_load_4d(v_smem(s) + c * Mma::kPiece, &map_v, v_full + 8 * s, c * 64, (first + it) * kHalf, hk * p.v_at.head, b * p.v_at.batch);
     };
     if (threadIdx.x == 0) {
-        ptx::mbar_init(q_full, 1); ptx::mbar_init(acc_full, 1); ptx::mbar_init(ml_ready, 8); ptx::mbar_init(staged, 8);
+        ptx::mbar_init(q_full, 1); ptx::mbar_init(acc_full, 1);
+        if (kQInTmem) ptx::mbar_init(q_ready, 8); ptx::mbar_init(ml_ready, 8); ptx::mbar_init(staged, 8);
         for (int y = 0; y < kBuffers; ++y) { ptx::mbar_init(s_full + 8 * y, 1); ptx::mbar_init(p_ready + 8 * y, 4); }
         ptx::mbar_init(o_done, 1); ptx::mbar_init(o_done + 8, 1);
         for (int s = 0; s < kStagesK; ++s) { ptx::mbar_init(k_full + 8 * s, 1); ptx::mbar_init(k_empty + 8 * s, 1); }
@@ -169,27 +173,30 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             const uint32_t lead = ptx::elect_lead();
             const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
             const int tiles = __shfl_sync(0xffffffffu, n_it, 0);
-            int ks = 0, vs = 0;
-            uint32_t k_phase = 0, v_phase = 0;
+            int ks = 0, vs = 0, next = 0, at = 0;               // stages; buffers of the next S and of tile it
+            uint32_t k_phase = 0, v_phase = 0, p_phase = 0;
             auto s_product = [&](int it) {
                 if (!warp_spin(wctx, k_full + 8 * ks, k_phase, 0x04030000u | (it & 0xffff))) return false;
                 ptx::tc_fence_after_sync();
-                Mma::scores_ss(lead, tmem + 64 * (it % kBuffers), q_smem, k_smem(ks));
-                ptx::mma_commit_lead(lead, s_full + 8 * (it % kBuffers));
+                if constexpr (kQInTmem) Mma::scores_ts(lead, tmem + 64 * next, tmem + kColQ, k_smem(ks));
+                else Mma::scores_ss(lead, tmem + 64 * next, q_smem, k_smem(ks));
+                ptx::mma_commit_lead(lead, s_full + 8 * next);
+                if (++next == kBuffers) next = 0;
                 ptx::mma_commit_lead(lead, k_empty + 8 * ks);
                 if (++ks == kStagesK) { ks = 0; k_phase ^= 1; }
                 return true;
             };
-            bool ok = tiles == 0 || warp_spin(wctx, q_full, 0, 0x04040000u);
+            bool ok = tiles == 0 || warp_spin(wctx, q_ready, 0, 0x04040000u);
             for (int it = 0; it < kBuffers && it < tiles && ok; ++it) ok = s_product(it);
             for (int it = 0; it < tiles && ok; ++it) {
                 if (!(ok = warp_spin(wctx, v_full + 8 * vs, v_phase, 0x04050000u | (it & 0xffff)))) break;
-                if (!(ok = warp_spin(wctx, p_ready + 8 * (it % kBuffers), (it / kBuffers) & 1, 0x04060000u | (it & 0xffff)))) break;
+                if (!(ok = warp_spin(wctx, p_ready + 8 * at, p_phase, 0x04060000u | (it & 0xffff)))) break;
                 ptx::tc_fence_after_sync();
-                Mma::grads(lead, tmem + kColO + D * (it & 1), tmem + 64 * (it % kBuffers), v_smem(vs), it < 2);
+                Mma::grads(lead, tmem + kColO + D * (it & 1), tmem + 64 * at, v_smem(vs), it < 2);
                 ptx::mma_commit_lead(lead, o_done + 8 * (it & 1));
                 ptx::mma_commit_lead(lead, v_empty + 8 * vs);
                 if (it + kBuffers < tiles && !(ok = s_product(it + kBuffers))) break;
+                if (++at == kBuffers) { at = 0; p_phase ^= 1; }
                 if (++vs == kStagesV) { vs = 0; v_phase ^= 1; }
             }
             if (ok) ptx::mma_commit_lead(lead, acc_full);
@@ -206,14 +213,23 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         float m_run = -CUDART_INF_F;      // the max the exponentials are taken against (log2 units)
         float l_run = 0.0f;
         bool ok = true;
+        if (kQInTmem && n_it > 0 && (ok = warp_wait(wctx, q_full, 0, 0x040d0000u))) {            // each group brings half of Q to tensor memory
+            row_to_tmem<D / 64>(tmem_base + lane_base + kColQ, q_smem, row_in_tile, x * (D / 64));
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(q_ready);
+        }
         WarpBias wb(p.h);
+        int buffer = x;                                         // of tile it
+        uint32_t buffer_phase = 0;
         for (int it = x; it < n_it && ok; it += 2) {
             const int key0 = (first + it) * kHalf;
-            const uint32_t s_at = tmem_base + lane_base + 64 * (it % kBuffers);
+            const uint32_t s_at = tmem_base + lane_base + 64 * buffer;
             float c = p.h.scale_log2, add = 0.0f;               // a score in log2 units is c * s + add
             bool looked_up = false;
             if constexpr (BIAS) looked_up = !wb.block(bias, bias.value, w, lane, p.h.n_runs, key0 - (row0 + quarter * 32 + 31 + offset));
-            ok = warp_wait(wctx, s_full + 8 * (it % kBuffers), (it / kBuffers) & 1, 0x04070000u | (it & 0xffff));
+            ok = warp_wait(wctx, s_full + 8 * buffer, buffer_phase, 0x04070000u | (it & 0xffff));
             if (!ok) break;
             ptx::tc_fence_after_sync();
             uint32_t r[64];
@@ -296,7 +312,9 @@ heads_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             ptx::tmem_st_wait();
             ptx::tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(p_ready + 8 * (it % kBuffers));
+            if (lane == 0) ptx::mbar_arrive(p_ready + 8 * buffer);
+            buffer += 2;
+            if (buffer >= kBuffers) { buffer -= kBuffers; buffer_phase ^= 1; }
         }
         // ---- the two groups joined; each writes half of the columns ----------------------------------------------------------
         if (ok) {

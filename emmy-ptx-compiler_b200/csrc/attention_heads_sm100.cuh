@@ -182,6 +182,24 @@ struct Products {
         for (int kk = 0; kk < kHalf / 16; ++kk) ptx::mma_ts_lead(lead, d, a + kk * 8, lo + ((kk * 16 * 128) >> 4), kHi, kGrads, !first || kk != 0);
     }
 };
+// Part of a row of a 128-row tile in shared memory (pieces of 128 rows x 64 elements, 128-byte swizzle) into tensor memory, as the A
+// operand of a product: columns of element pairs. Elements 32 first .. 32 (first + N) - 1; `taddr`: of the row's first element. (Threads
+// reading their rows from global memory instead took 7000 cycles of a CTA's set-up.)
+template <int N>
+__device__ __forceinline__ void row_to_tmem(uint32_t taddr, uint32_t tile, int row, int first = 0) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int i = first + n;
+        uint32_t r[16];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int piece = (i % 2) * 4 + k;
+            ptx::ld_shared_16B(tile + (i / 2) * (kTile * 128) + row * 128 + ((piece ^ (row & 7)) << 4), r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+        }
+        ptx::tmem_st_32x32b_x16(taddr + 16 * i, r);
+    }
+}
+
 // ---- the order of the work items -----------------------------------------------------------------------------------------------
 // Causal tiles differ in length. Dealt longest first over many units the SMs finish together; dealt unit by unit the last units'
 // longest tiles run alone (16 units of 2048 keys on 148 SMs: 184 us against 118). But CTAs that run at the same time should share
