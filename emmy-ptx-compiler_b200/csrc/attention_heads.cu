@@ -280,7 +280,7 @@ extern "C" int64_t emmyb200_attention_heads_workspace_bytes(const emmyb200_atten
     if (check_desc(c, backward != 0, "attention_heads_workspace_bytes") != EMMYB200_OK) return -1;
     if (backward) return bwd_layout(c).total;
     if (c->batch * c->heads * c->seq_q * c->seq_k == 0 || c->dtype == EMMYB200_F32 || (c->d != 64 && c->d != 128)) return 0;
-    return fwd_workspace(heads_fwd_plan(make_params(c, nullptr, nullptr)), c->d);
+    return fwd_workspace(heads_fwd_plan(make_params(c, nullptr, nullptr), c->d), c->d);
 }
 
 extern "C" int emmyb200_attention_heads_fwd(const emmyb200_attention_heads_desc* c, const void* Q, const void* K, const void* V,
@@ -299,7 +299,7 @@ extern "C" int emmyb200_attention_heads_fwd(const emmyb200_attention_heads_desc*
     if (rc != EMMYB200_OK) return rc;
     const HeadsParams p = make_params(c, key_lens, table);
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-    if (heads_sm100_takes(p, c->dtype, (int)c->d, Q, K, V, O)) return heads_fwd_sm100(c->dtype, (int)c->d, p, heads_fwd_plan(p), Q, K, V, O, lse, workspace, s);
+    if (heads_sm100_takes(p, c->dtype, (int)c->d, Q, K, V, O)) return heads_fwd_sm100(c->dtype, (int)c->d, p, heads_fwd_plan(p, c->d), Q, K, V, O, lse, workspace, s);
     return heads_fwd_cores(c->dtype, (int)c->d, p, Q, K, V, O, lse, s);
 }
 

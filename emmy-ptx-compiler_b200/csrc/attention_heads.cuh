@@ -91,7 +91,7 @@ struct FwdPlan {
     int packed, tiles, splits;                  // see attention_heads_fwd_sm100.cu
     int64_t rows;                               // batch * heads * seq_q
 };
-FwdPlan heads_fwd_plan(const HeadsParams& p);
+FwdPlan heads_fwd_plan(const HeadsParams& p, int64_t d);
 // Workspace of split keys: float2[splits][rows], then float[splits][rows][d].
 inline int64_t fwd_part_offset(const FwdPlan& w) { return (w.splits * w.rows * 8 + 255) / 256 * 256; }
 inline int64_t fwd_workspace(const FwdPlan& w, int64_t d) { return w.splits == 1 ? 0 : (fwd_part_offset(w) + w.splits * w.rows * d * 4 + 255) / 256 * 256; }

@@ -461,17 +461,18 @@ static int launch(FwdParams& p, const FwdPlan& plan, const void* Q, const void* 
 
 }  // namespace heads
 
-FwdPlan heads_fwd_plan(const HeadsParams& p) {
+FwdPlan heads_fwd_plan(const HeadsParams& p, int64_t d) {
     FwdPlan plan;
     // Packed rows: worth it whenever they fit one tile, since the tile's cost does not depend on how many of its rows are used. Not
     // with a bias (its values belong to a head), nor over broadcast query heads (no dimension to load them along).
     plan.packed = p.group > 1 && (int64_t)p.group * p.seq_q <= heads::kTile && p.n_runs == 0 && p.q_s[1] != 0;
     plan.tiles = plan.packed ? 1 : (p.seq_q + heads::kTile - 1) / heads::kTile;
     const int64_t items = (int64_t)p.batch * (plan.packed ? p.kv_heads : p.heads) * plan.tiles;
-    // Splitting the keys costs a second launch and a set-up per CTA: worth it while there is less than one tile per SM (256 tiles
-    // of 64 key tiles each: 152 us whole, 171 us in two; 32 tiles: 126 us whole, 35 us in eight; 8 tiles: 121 us whole, 22 us in
-    // sixteen). Then as many CTAs as are resident at once, of at least four key tiles each, none of them shorter than it has to be.
-    const int64_t key_tiles = (p.seq_k + heads::kTile - 1) / heads::kTile, slots = 2 * sm_count();
+    // Splitting the keys costs a second launch and a set-up per CTA: worth it while there is less than one tile per SM (caches of 8192
+    // keys, d = 128: 256 tiles 140 us whole, 145 us in two; 32 tiles 60 us whole, 33 us in four, 36 us in eight; 8 tiles 57 us whole, 21 us in
+    // eight to sixteen). Then at most as many CTAs as are resident at once, of at least four times 128 keys each, none of them shorter
+    // than it has to be.
+    const int64_t key_tiles = (p.seq_k + heads::kTile - 1) / heads::kTile, slots = (d == 64 ? 2 : 1) * sm_count();
     plan.splits = 1;
     if (items < sm_count()) {
         const int64_t most = std::max<int64_t>(1, std::min<int64_t>(slots / items, key_tiles / 4));
