@@ -57,6 +57,13 @@ __device__ __forceinline__ uint32_t operand_pair(float2 v) {
     else return round_pair<false>(v.x, v.y);
 }
 
+// The same rounded (half a step away from zero on a tie): two additions more per pair.
+template <bool BF16>
+__device__ __forceinline__ uint32_t rounded_pair(float2 v) {
+    if constexpr (BF16) return __byte_perm(__float_as_uint(v.x) + 0x8000u, __float_as_uint(v.y) + 0x8000u, 0x7632);
+    else return round_pair<false>(v.x, v.y);
+}
+
 // ---- waits of a whole warp ---------------------------------------------------------------------------------------------------
 // One poll by all lanes and a vote is the common case and costs some 50 cycles less than a loop per lane around it (the
 // issuing warp makes three or four waits per tile: with the per-lane form they took longer than the products). The limit and the
