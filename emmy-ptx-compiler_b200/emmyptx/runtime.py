@@ -706,6 +706,8 @@ class _Switched:
         self.guards = []
         if device.type != "cuda":                   # refused with the reason when the call is checked
             return
+        if stream is not None and stream.device != device:
+            raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
         if torch.cuda.current_device() != device.index:
             self.guards.append(torch.cuda.device(device))
         if stream is not None:
